@@ -20,6 +20,8 @@ from pathlib import Path
 import torch
 import torch.nn.functional as F
 
+sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "tt-rl_amd"))
+
 own = False
 
 CHUNK = 64  # steps of the plain form's chunks
@@ -336,9 +338,6 @@ def _split(flat, state) -> list:
 # ------------------------------------------------------------- the package ---
 
 def _device():
-    root = str(Path(__file__).resolve().parents[1] / "tt-rl_amd")
-    if root not in sys.path:
-        sys.path.insert(0, root)
     from ttrl_amd.engine.device import open_device
 
     return open_device(0)
