@@ -828,6 +828,113 @@ int ttrl_gru_step_backward_ragged(ttrl_ctx* ctx, int B, int H, const float* dgh,
                                   const float* dout_prev, const float* done, float* dgi_prev, float* dgh_prev,
                                   float* dhz_prev);
 
+/* ---- sequence policies ------------------------------------------------------ */
+
+/* Linear attention with a decay for each head, the recurrent memory of a
+ * sequence policy (no counterpart in the reference, whose memory is a GRU;
+ * rows are time-major and `done` resets the state entering a step, as there):
+ *   S_t = a_t S_{t-1} + k_t v_t^T,  o_t = scale q_t^T S_t,  a_t = exp(log decay),
+ *   a_t = 0 where done[t] > 0 (or the decay underflows).
+ * q, dq [T][B][H][K]; k, dk [T][B][kv_heads][K]; v, dv [T][B][kv_heads][V], head
+ * h using key/value head h / (H / kv_heads); out, dout [T][B][H][V]; log_decay
+ * and dlog_decay [T][B][H] with decay_steps, else [H]; done [T][B] or NULL;
+ * state (NULL: zeros), final_state, dfinal (NULL: zeros), dstate (NULL: not
+ * wanted) [B][H][K][V].  K and V up to 128; T and B may be 0.
+ * Nothing that is not finite passes from one episode to another, or to an
+ * earlier output.
+ * ttrl_linear_attention_space: floats of `saved`, which the forward fills for
+ * the backward, and of `work`, which the backward uses; both may then be
+ * NULL where 0.  The backward overwrites dq, dk and dv (all required) and
+ * dlog_decay unless NULL; with dlog_decay and dfinal it reads final_state. */
+typedef struct ttrl_linear_attention_desc {
+  int T, B, H, kv_heads, K, V;
+  const float* q;
+  const float* k;
+  const float* v;
+  const float* log_decay;
+  int decay_steps;
+  const float* done;
+  float scale;
+  const float* state;
+  float* out;
+  float* final_state;
+  float* saved;
+  float* work;
+  const float* dout;
+  const float* dfinal;
+  float* dq;
+  float* dk;
+  float* dv;
+  float* dlog_decay;
+  float* dstate;
+} ttrl_linear_attention_desc;
+int ttrl_linear_attention_space(const ttrl_linear_attention_desc* desc, long* saved_floats, long* work_floats);
+int ttrl_linear_attention_forward(ttrl_ctx* ctx, const ttrl_linear_attention_desc* desc);
+int ttrl_linear_attention_backward(ttrl_ctx* ctx, const ttrl_linear_attention_desc* desc);
+/* One token of B lanes: state [B][H][K][V] is stepped in place, out [B][H][V];
+ * q [B][H][K], k [B][kv_heads][K], v [B][kv_heads][V], log_decay [B][H] with
+ * decay_rows, else [H]; done [B] or NULL. */
+int ttrl_linear_attention_token(ttrl_ctx* ctx, int B, int H, int kv_heads, int K, int V, const float* q, const float* k,
+                                const float* v, const float* log_decay, int decay_rows, const float* done, float scale,
+                                float* state, float* out);
+
+/* The gated projections of a feed-forward block (no counterpart in the
+ * reference): h = act(x W_gate + b_gate) * (x W_up + b_up), x [M][K], weights
+ * [K][N] (in, out), biases [N] or NULL, h [M][N].  g and u, both or neither,
+ * receive the two projections for the backward.  act: */
+#define TTRL_GATE_SILU 0
+#define TTRL_GATE_GELU 1 /* with the error function */
+#define TTRL_GATE_RELU 2
+#define TTRL_GATE_SIGMOID 3
+typedef struct ttrl_gated_desc {
+  int M, K, N, act;
+  const float* x;
+  const float* w_gate;
+  const float* w_up;
+  const float* b_gate;
+  const float* b_up;
+  float* g;
+  float* u;
+  float* h;
+} ttrl_gated_desc;
+int ttrl_gated_forward(ttrl_ctx* ctx, const ttrl_gated_desc* desc);
+/* dg = dh * u * act'(g), du = dh * act(g), all [M][N]. */
+int ttrl_gated_slopes(ttrl_ctx* ctx, int M, int N, int act, const float* dh, const float* g, const float* u, float* dg,
+                      float* du);
+
+/* AdamW over many tensors in one launch per 64 (the reference's Adam,
+ * ttrl/engine/optim/adam.py:25-134, has coupled decay and 32-bit states):
+ *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
+ *   p = (1 - lr wd) p - (lr / bc1) m / (sqrt(v) / sqrt(bc2) + eps).
+ * Tensor i's moments are elements [at, at + n) of m and v (floats on 16 bytes),
+ * at a multiple of 64.  state_bits 8: m holds a signed and v an unsigned byte
+ * per element, and m_scale and v_scale [at / 64 ..] each block's largest
+ * magnitude; m's code c stands for c |c| / 127^2 scale, v's for (c / 255)^4 scale;
+ * the buffers hold whole blocks for every tensor.  A moment that is not
+ * finite spoils its block.
+ * counter: TTRL_ADAMW_COUNTER_BYTES of device memory, set by
+ * ttrl_adamw_set_count (t updates done) and moved on by every step. */
+#define TTRL_ADAMW_COUNTER_BYTES 24
+typedef struct ttrl_adamw_tensor {
+  float* p;
+  const float* g;
+  long at;
+  long n;
+} ttrl_adamw_tensor;
+typedef struct ttrl_adamw_moment {
+  float* m;
+  float* v;
+  long at;
+  long n;
+} ttrl_adamw_moment;
+int ttrl_adamw_set_count(ttrl_ctx* ctx, void* counter, int t, double beta1, double beta2);
+int ttrl_adamw_step(ttrl_ctx* ctx, int count, const ttrl_adamw_tensor* tensors, int state_bits, void* m, void* v,
+                    float* m_scale, float* v_scale, void* counter, double lr, double beta1, double beta2, double eps,
+                    double weight_decay);
+/* The values that 8-bit moments stand for, written to each tensor's m and v. */
+int ttrl_adamw_moments(ttrl_ctx* ctx, int count, const ttrl_adamw_moment* tensors, const void* m, const void* v,
+                       const float* m_scale, const float* v_scale);
+
 /* ---- GPU-resident replay -------------------------------------------------- */
 
 /* One replay ring in device memory (ttrl/buffers/replay.py:62-129): per lane

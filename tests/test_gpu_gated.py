@@ -1,0 +1,206 @@
+"""The gated projections on the GPU against the float64 oracle: outputs and
+every gradient over rows, widths, activations and alignments.
+
+Tolerance, from float32's rounding before the first run (u = 2^-24): a
+projection's error is at most (K + 8) u times the sum of its absolute terms,
+P.  All four activations have slopes and second derivatives of at most 1.2, so
+h = act(g) u is off by at most (K + 16) u (1.2 P_g |u| + |act| P_u + |h|), and dg and
+du by the same with dh; their errors and (M or N + 8) u of the absolute terms
+add up in the products that follow."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from oracle import sequence as O
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _tensor(device, a, grad=True, offset=0):
+    from ttrl_amd.engine.autograd import Tensor
+    from ttrl_amd.engine.tensor import DeviceArray
+
+    view = DeviceArray(device, (a.size + offset,)).view(offset, a.shape)
+    view.upload(a)
+    return Tensor(view, grad)
+
+
+def _inputs(seed, M, K, N, bias):
+    rng = np.random.default_rng(seed)
+
+    def normal(*s, scale=1.0):
+        return (scale * rng.standard_normal(s)).astype(np.float32)
+
+    x = {"x": normal(M, K), "w_gate": normal(K, N, scale=K ** -0.5), "w_up": normal(K, N, scale=K ** -0.5),
+         "b_gate": normal(1, N) if bias else None, "b_up": normal(1, N) if bias else None}
+    return x, normal(M, N)
+
+
+def _run(device, x, act, dh, offset=0):
+    from ttrl_amd.engine.autograd import backward_from
+    from ttrl_amd.engine.ops import gated_linear
+
+    t = {n: None if a is None else _tensor(device, a, True, offset) for n, a in x.items()}
+    h = gated_linear(*t.values(), activation=act)
+    got = {"out": h.numpy()}
+    backward_from([(h, _tensor(device, dh, False, offset))])
+    got.update({n: a.grad.numpy() for n, a in t.items() if a is not None})
+    return got
+
+
+def _bounds(x, act, dh):
+    f = {n: None if a is None else a.astype(np.float64) for n, a in x.items()}
+    size = {n: 0.0 if a is None else np.abs(a) for n, a in f.items()}
+    (M, K), N = f["x"].shape, f["w_gate"].shape[1]
+    g, u = O._projections(f["x"], f["w_gate"], f["w_up"], f["b_gate"], f["b_up"])
+    pg, pu = size["x"] @ size["w_gate"] + size["b_gate"], size["x"] @ size["w_up"] + size["b_up"]
+    a, slope = O._act(act, g)
+    d = np.abs(dh.astype(np.float64))
+    n = (K + 16) * U
+    out = n * (1.2 * pg * np.abs(u) + np.abs(a) * pu + np.abs(a * u) + 1e-30)
+    eg = n * d * (1.2 * pg * np.abs(u) + 1.2 * pu + np.abs(slope * u))  # of dg
+    eu = n * d * (1.2 * pg + np.abs(a))  # of du
+    ag, au = d * np.abs(u * slope), d * np.abs(a)
+    xt = size["x"].T
+    return {"out": out, "w_gate": xt @ (eg + (M + 8) * U * ag), "w_up": xt @ (eu + (M + 8) * U * au),
+            "b_gate": (eg + (M + 8) * U * ag).sum(0, keepdims=True), "b_up": (eu + (M + 8) * U * au).sum(0, keepdims=True),
+            "x": (eg + (2 * N + 8) * U * ag) @ size["w_gate"].T + (eu + (2 * N + 8) * U * au) @ size["w_up"].T}
+
+
+def _check(got, x, act, dh):
+    want = O.gated_backward(*x.values(), act, dh)
+    want["out"] = O.gated_forward(*x.values(), act)
+    lim = _bounds(x, act, dh)
+    for n, a in got.items():
+        err = np.abs(a.astype(np.float64) - want[n])
+        assert a.shape == want[n].shape, n
+        assert (err <= lim[n] + 1e-30).all(), (n, float((err / (lim[n] + 1e-30)).max()))
+
+
+SIZES = [(1, 1, 1), (1, 512, 2048), (2, 64, 100), (5, 33, 7), (16, 500, 64), (17, 16, 65), (64, 128, 64), (65, 31, 129),
+         (200, 100, 333), (1000, 72, 60)]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu", "sigmoid"])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_matches_the_oracle(device, M, K, N, act):
+    x, dh = _inputs(M + K + N, M, K, N, bias=(M + N) % 2 == 1)
+    if act == "relu":  # a gate that rounding decides has no float64 value
+        g = O._projections(*x.values())[0]
+        dh[np.abs(g) < 1e-4] = 0
+    _check(_run(device, x, act, dh), x, act, dh)
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_any_alignment(device, offset):
+    for M in (1, 70):
+        x, dh = _inputs(offset, M, 48, 96, bias=True)
+        _check(_run(device, x, "silu", dh, offset), x, "silu", dh)
+
+
+def test_large_rows(device):
+    """Rows and widths of a training batch (the matrix-core path)."""
+    x, dh = _inputs(5, 2050, 260, 516, bias=True)
+    _check(_run(device, x, "gelu", dh), x, "gelu", dh)
+
+
+def test_extreme_projections(device):
+    """Gates far from zero saturate, they do not turn into NaN."""
+    x, dh = _inputs(6, 3, 4, 8, bias=True)
+    x["b_gate"][0, :4] = [200, -200, 1e4, -1e4]
+    for act in ("silu", "gelu", "sigmoid"):
+        got = _run(device, x, act, dh)
+        assert all(np.isfinite(a).all() for a in got.values()), act
+        want = O.gated_forward(*x.values(), act)
+        assert np.allclose(got["out"], want, rtol=1e-4, atol=1e-5), act
+
+
+@pytest.mark.parametrize("M", [3, 300])
+def test_what_is_not_finite_stays_in_its_row(device, M):
+    x, dh = _inputs(7, M, 32, 64, bias=False)
+    clean = _run(device, x, "silu", dh)
+    for bad in (np.nan, np.inf):
+        y = {n: None if a is None else a.copy() for n, a in x.items()}
+        y["x"][2, 5] = bad
+        got = _run(device, y, "silu", dh)
+        for n in ("out", "x"):
+            rest = np.delete(np.arange(M), 2)
+            assert np.array_equal(got[n][rest], clean[n][rest]), n
+        assert not np.isfinite(got["out"][2]).any()
+
+
+def test_no_rows_and_no_tape(device):
+    from ttrl_amd.engine.autograd import no_grad
+    from ttrl_amd.engine.ops import gated_linear
+
+    x, dh = _inputs(8, 0, 8, 12, bias=True)
+    got = _run(device, x, "silu", dh)
+    assert got["out"].shape == (0, 12) and not any(got[n].any() for n in ("w_gate", "w_up", "b_gate", "b_up"))
+    x, dh = _inputs(9, 40, 8, 12, bias=True)
+    with no_grad():
+        h = gated_linear(*(_tensor(device, a) for a in x.values()))
+    assert not h.requires_grad and np.array_equal(h.numpy(), _run(device, x, "silu", dh)["out"])
+
+
+def test_gradients_add_and_bias_alone(device):
+    from ttrl_amd.engine.autograd import backward_from
+    from ttrl_amd.engine.ops import gated_linear
+
+    x, dh = _inputs(10, 30, 20, 24, bias=True)
+    t = {n: _tensor(device, a) for n, a in x.items()}
+    for _ in range(2):
+        backward_from([(gated_linear(*t.values(), activation="gelu"), _tensor(device, dh, False))])
+    want = O.gated_backward(*x.values(), "gelu", dh)
+    lim = _bounds(x, "gelu", dh)
+    for n, a in t.items():
+        assert (np.abs(a.grad.numpy() - 2 * want[n]) <= 2 * lim[n] + 8 * U * np.abs(want[n])).all(), n
+    only = {n: _tensor(device, a, n.startswith("b_")) for n, a in x.items()}
+    backward_from([(gated_linear(*only.values(), activation="gelu"), _tensor(device, dh, False))])
+    for n in ("b_gate", "b_up"):
+        assert (np.abs(only[n].grad.numpy() - want[n]) <= lim[n]).all(), n
+    assert only["x"].grad is None and only["w_gate"].grad is None
+
+
+def test_a_captured_pass_replays(device):
+    from ttrl_amd.engine.autograd import backward_from
+    from ttrl_amd.engine.ops import gated_linear
+    from ttrl_amd.engine.step import TrainStep
+
+    x, dh = _inputs(11, 130, 40, 72, bias=True)
+    eager = _run(device, x, "silu", dh)
+    t = {n: _tensor(device, a) for n, a in x.items()}
+    seed = _tensor(device, dh, False)
+    made = {}
+
+    def body(t):
+        for a in t.values():
+            a.zero_grad()
+        made["h"] = gated_linear(*t.values())
+        backward_from([(made["h"], seed)])
+        return {}
+
+    with TrainStep(body, t, device, mode="graph") as step:
+        step.run()
+        for _ in range(3):
+            step.replay()
+            device.synchronize()
+            assert np.array_equal(made["h"].numpy(), eager["out"])
+            for n, a in t.items():
+                assert np.array_equal(a.grad.numpy(), eager[n]), n
+
+
+def test_refusals(device):
+    from ttrl_amd.engine.ops import gated_linear
+
+    def t(*shape):
+        return _tensor(device, np.zeros(shape, np.float32))
+
+    for bad in ((t(2, 3), t(4, 5), t(4, 5)), (t(2, 4), t(4, 5), t(4, 6)), (t(2, 4), t(4, 5), t(4, 5), t(1, 4)),
+                (t(8), t(4, 5), t(4, 5))):
+        with pytest.raises(ValueError):
+            gated_linear(*bad)
+    with pytest.raises(ValueError):
+        gated_linear(t(2, 4), t(4, 5), t(4, 5), activation="tanh")

@@ -1,0 +1,359 @@
+// AdamW over many tensors at once (Loshchilov and Hutter, "Decoupled Weight
+// Decay Regularization", ICLR 2019), moments in 32 bits or in 8:
+//
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
+//   p = (1 - lr wd) p - (lr / bc1) m / (sqrt(v) / sqrt(bc2) + eps),  bci = 1 - bi^t.
+//
+// In 8 bits a moment is a code per element and a scale per block of 64
+// elements, the block's largest magnitude (block-wise scales after Dettmers et
+// al., "8-bit Optimizers via Block-wise Quantization", ICLR 2022; the codes
+// are this file's own): m's code c is the nearest of 127 signed steps of
+// sqrt(|m| / scale) and stands for c |c| / 127^2 scale, v's the nearest of 255
+// steps of the fourth root and stands for (c / 255)^4 scale.  The roots spend
+// the codes on small values (v down to 2.4e-10 of its block's largest, which
+// squares of gradients reach), and a v that is not zero is held as at least
+// code 1, so no step is ever divided by eps alone.  The update itself uses the
+// new moments before they are rounded to codes.
+//
+// Each product and sum is rounded on its own (no contraction into FMAs), so
+// that 32-bit states, 8-bit codes and parameters are the same bits however the
+// compiler schedules the kernel.
+//
+// One launch takes up to 64 tensors: their addresses travel in the kernel's
+// arguments, so the step can be captured into a graph and no table is uploaded.
+// A workgroup takes kSpan elements of one tensor, found by bisection over the
+// tensors' first workgroups.  Bound: HBM, 28 bytes a parameter in 32 bits,
+// 16.25 in 8 (4 + 4 + 4 of p and g, 2 + 2 of codes, 0.25 of scales).
+//
+// The update count and the next update's bias corrections live on the device;
+// the last workgroup of a step's last launch moves them on, so a replayed
+// graph counts by itself and no workgroup waits for the powers.
+#include "common.hpp"
+
+#include <algorithm>
+
+namespace ttrl {
+namespace {
+
+constexpr int kThreads = 256, kRounds = 4, kSpan = kThreads * 4 * kRounds;
+constexpr int kTensors = 64, kBlock = 64;
+
+struct Counter {
+  int t;             // updates done
+  unsigned tickets;  // workgroups of the running launch that are done
+  double bc1, root;  // 1 - b1^(t+1) and 1 / sqrt(1 - b2^(t+1))
+};
+static_assert(sizeof(Counter) == TTRL_ADAMW_COUNTER_BYTES, "the size callers allocate");
+
+__device__ void set_count(Counter* c, int t, double b1, double b2) {
+  c->t = t;
+  c->tickets = 0;
+  c->bc1 = 1.0 - pow(b1, double(t + 1));
+  c->root = 1.0 / sqrt(1.0 - pow(b2, double(t + 1)));
+}
+
+__global__ void k_adamw_set(Counter* c, int t, double b1, double b2) { set_count(c, t, b1, b2); }
+
+struct Item {
+  float* p;
+  const float* g;
+  long at, n;  // its place in the moments, its elements
+  int first;   // its first workgroup
+  int wide;    // p and g on 16 bytes
+};
+struct AdamWArgs {
+  Item item[kTensors];
+  int count;
+  void *m, *v;
+  float *m_scale, *v_scale;
+  Counter* counter;
+  double lr, b1d, b2d;
+  float b1, c1, b2, c2, eps, shrink;
+  int last;  // the step's last launch
+};
+
+__device__ __forceinline__ f32x4 load4(const float* p, long i, long n, bool whole) {
+  if (whole) return *reinterpret_cast<const f32x4*>(p + i);
+  f32x4 x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = i + j < n ? p[i + j] : 0.f;
+  return x;
+}
+__device__ __forceinline__ void store4(float* p, long i, long n, bool whole, const f32x4& x) {
+  if (whole) {
+    *reinterpret_cast<f32x4*>(p + i) = x;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (i + j < n) p[i + j] = x[j];
+}
+
+// The largest over the 16 lanes (a DPP row) that hold a block.
+__device__ __forceinline__ float row_max(float x) {
+#define TTRL_ROW_ROR(n) \
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + n, 0xf, 0xf, true)))
+  TTRL_ROW_ROR(8);
+  TTRL_ROW_ROR(4);
+  TTRL_ROW_ROR(2);
+  TTRL_ROW_ROR(1);
+#undef TTRL_ROW_ROR
+  return x;
+}
+
+__device__ __forceinline__ float held_m(int code, float scale) {
+#pragma clang fp contract(off)
+  const float c = float(code) * (1.f / 127.f);
+  return c * fabsf(c) * scale;
+}
+__device__ __forceinline__ float held_v(unsigned code, float scale) {
+#pragma clang fp contract(off)
+  float c = float(code) * (1.f / 255.f);
+  c = c * c;
+  return c * c * scale;
+}
+__device__ __forceinline__ int code_m(float m, float scale) {
+#pragma clang fp contract(off)
+  const float r = scale > 0.f ? fabsf(m) / scale : 0.f;
+  const int c = int(rintf(sqrtf(r) * 127.f));
+  return m < 0.f ? -c : c;
+}
+__device__ __forceinline__ unsigned code_v(float v, float scale) {
+#pragma clang fp contract(off)
+  const float r = scale > 0.f ? v / scale : 0.f;
+  const float c = rintf(sqrtf(sqrtf(r)) * 255.f);
+  return unsigned(r > 0.f ? fmaxf(c, 1.f) : c);
+}
+
+__device__ __forceinline__ int item_of(const AdamWArgs& a, int block) {
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (block >= a.item[mid].first) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <bool HELD>
+__global__ __launch_bounds__(kThreads) void k_adamw(AdamWArgs a) {
+#pragma clang fp contract(off)
+  const Item& it = a.item[item_of(a, int(blockIdx.x))];
+  const long from = long(int(blockIdx.x) - it.first) * kSpan + threadIdx.x * 4, n = it.n;
+  const double bc1 = a.counter->bc1, root64 = a.counter->root;
+  f32x4 p[kRounds], g[kRounds], m[kRounds], v[kRounds];
+  uint32_t mc[kRounds], vc[kRounds];
+  float ms[kRounds], vs[kRounds];
+  bool in[kRounds], whole[kRounds];
+#pragma unroll
+  for (int u = 0; u < kRounds; ++u) {
+    const long i = from + u * (kThreads * 4), s = it.at + i;
+    in[u] = i < n;
+    whole[u] = it.wide && i + 4 <= n;
+    if (!in[u]) continue;
+    p[u] = load4(it.p, i, n, whole[u]);
+    g[u] = load4(it.g, i, n, whole[u]);
+    if constexpr (HELD) {  // a tensor's moments end on a block: whole reads
+      mc[u] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.m) + s);
+      vc[u] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + s);
+      ms[u] = a.m_scale[s / kBlock];
+      vs[u] = a.v_scale[s / kBlock];
+    } else {
+      m[u] = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.m) + s);
+      v[u] = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.v) + s);
+    }
+  }
+  const float size = float(a.lr / bc1), root = float(root64);
+#pragma unroll
+  for (int u = 0; u < kRounds; ++u) {
+    const long i = from + u * (kThreads * 4), s = it.at + i;
+    float top_m = 0.f, top_v = 0.f;
+    if (in[u]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float mj, vj;
+        if constexpr (HELD) {
+          mj = held_m(int(int8_t(mc[u] >> (8 * j))), ms[u]);
+          vj = held_v(uint8_t(vc[u] >> (8 * j)), vs[u]);
+        } else {
+          mj = m[u][j];
+          vj = v[u][j];
+        }
+        const float gj = g[u][j];
+        mj = mj * a.b1 + gj * a.c1;
+        vj = vj * a.b2 + (gj * gj) * a.c2;
+        const float step = mj / (sqrtf(vj) * root + a.eps) * size;
+        p[u][j] = p[u][j] * a.shrink - step;
+        if (HELD && i + j >= n) mj = vj = 0.f;
+        m[u][j] = mj;
+        v[u][j] = vj;
+        top_m = fmaxf(top_m, fabsf(mj));
+        top_v = fmaxf(top_v, vj);
+      }
+      store4(it.p, i, n, whole[u], p[u]);
+      if constexpr (!HELD) {
+        store4(static_cast<float*>(a.m) + it.at, i, n, i + 4 <= n, m[u]);
+        store4(static_cast<float*>(a.v) + it.at, i, n, i + 4 <= n, v[u]);
+      }
+    }
+    if constexpr (HELD) {  // every lane of a row takes part
+      top_m = row_max(top_m);
+      top_v = row_max(top_v);
+      if (in[u]) {
+        uint32_t cm = 0, cv = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          cm |= (uint32_t(code_m(m[u][j], top_m)) & 255u) << (8 * j);
+          cv |= (code_v(v[u][j], top_v) & 255u) << (8 * j);
+        }
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + s) = cm;
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + s) = cv;
+        if ((threadIdx.x & 15) == 0) {
+          a.m_scale[s / kBlock] = top_m;
+          a.v_scale[s / kBlock] = top_v;
+        }
+      }
+    }
+  }
+  if (!a.last) return;
+  // Every workgroup has read the corrections before it takes its ticket.
+  __syncthreads();
+  if (threadIdx.x == 0 && atomicAdd(&a.counter->tickets, 1u) == gridDim.x - 1)
+    set_count(a.counter, a.counter->t + 1, a.b1d, a.b2d);
+}
+
+struct HeldItem {
+  float *m, *v;
+  long at, n;
+  int first;
+};
+struct HeldArgs {
+  HeldItem item[kTensors];
+  int count;
+  const uint8_t *mc, *vc;
+  const float *ms, *vs;
+};
+
+// The values that the codes stand for.
+__global__ __launch_bounds__(kThreads) void k_adamw_held(HeldArgs a) {
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (int(blockIdx.x) >= a.item[mid].first) lo = mid;
+    else hi = mid - 1;
+  }
+  const HeldItem& it = a.item[lo];
+  const long from = long(int(blockIdx.x) - it.first) * kSpan + threadIdx.x * 4;
+#pragma unroll
+  for (int u = 0; u < kRounds; ++u) {
+    const long i = from + u * (kThreads * 4), s = it.at + i;
+    if (i >= it.n) continue;
+    const uint32_t mc = *reinterpret_cast<const uint32_t*>(a.mc + s), vc = *reinterpret_cast<const uint32_t*>(a.vc + s);
+    const float ms = a.ms[s / kBlock], vs = a.vs[s / kBlock];
+    f32x4 m, v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = held_m(int(int8_t(mc >> (8 * j))), ms);
+      v[j] = held_v(uint8_t(vc >> (8 * j)), vs);
+    }
+    const bool whole = i + 4 <= it.n;
+    store4(it.m, i, it.n, whole && (reinterpret_cast<uintptr_t>(it.m) & 15) == 0, m);
+    store4(it.v, i, it.n, whole && (reinterpret_cast<uintptr_t>(it.v) & 15) == 0, v);
+  }
+}
+
+int blocks_of(long n) { return int((n + kSpan - 1) / kSpan); }
+
+}  // namespace
+}  // namespace ttrl
+
+using namespace ttrl;
+
+extern "C" {
+
+int ttrl_adamw_set_count(ttrl_ctx* ctx, void* counter, int t, double beta1, double beta2) {
+  TTRL_REQUIRE(ctx && counter, "ttrl_adamw_set_count: null argument");
+  TTRL_REQUIRE(t >= 0 && beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0,
+               "ttrl_adamw_set_count: t=%d, betas %g and %g", t, beta1, beta2);
+  hipLaunchKernelGGL(k_adamw_set, dim3(1), dim3(1), 0, stream_of(ctx), static_cast<Counter*>(counter), t, beta1, beta2);
+  return check_launch("ttrl_adamw_set_count");
+}
+
+int ttrl_adamw_step(ttrl_ctx* ctx, int count, const ttrl_adamw_tensor* tensors, int state_bits, void* m, void* v,
+                    float* m_scale, float* v_scale, void* counter, double lr, double beta1, double beta2, double eps,
+                    double weight_decay) {
+  const char* name = "ttrl_adamw_step";
+  TTRL_REQUIRE(ctx && tensors && m && v && counter, "%s: null argument", name);
+  TTRL_REQUIRE(count > 0, "%s: no tensors", name);
+  TTRL_REQUIRE(state_bits == 32 || state_bits == 8, "%s: moments in 32 or 8 bits, not %d", name, state_bits);
+  TTRL_REQUIRE(state_bits == 32 || (m_scale && v_scale), "%s: null scales", name);
+  TTRL_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "%s: betas %g and %g", name, beta1, beta2);
+  TTRL_REQUIRE(((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15) == 0,
+               "%s: moments must be 16-byte aligned", name);
+  for (int i = 0; i < count; ++i)
+    TTRL_REQUIRE(tensors[i].p && tensors[i].g && tensors[i].n > 0 && tensors[i].n <= (1L << 40) && tensors[i].at >= 0 &&
+                     tensors[i].at % kBlock == 0,
+                 "%s: tensor %d: null, empty, or its moments do not start on a block of %d", name, i, kBlock);
+  for (int from = 0; from < count; from += kTensors) {
+    AdamWArgs a{};
+    a.count = std::min(kTensors, count - from);
+    long blocks = 0;
+    for (int i = 0; i < a.count; ++i) {
+      const ttrl_adamw_tensor& t = tensors[from + i];
+      const bool wide = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g)) & 15) == 0;
+      a.item[i] = {t.p, t.g, t.at, t.n, int(blocks), wide};
+      blocks += blocks_of(t.n);
+      TTRL_REQUIRE(blocks <= 0x7fffffffL, "%s: too many elements", name);
+    }
+    a.m = m;
+    a.v = v;
+    a.m_scale = m_scale;
+    a.v_scale = v_scale;
+    a.counter = static_cast<Counter*>(counter);
+    a.lr = lr;
+    a.b1d = beta1;
+    a.b2d = beta2;
+    a.b1 = float(beta1);
+    a.c1 = float(1.0 - beta1);
+    a.b2 = float(beta2);
+    a.c2 = float(1.0 - beta2);
+    a.eps = float(eps);
+    a.shrink = float(1.0 - lr * weight_decay);
+    a.last = from + kTensors >= count;
+    if (state_bits == 8) hipLaunchKernelGGL(k_adamw<true>, dim3(unsigned(blocks)), dim3(kThreads), 0, stream_of(ctx), a);
+    else hipLaunchKernelGGL(k_adamw<false>, dim3(unsigned(blocks)), dim3(kThreads), 0, stream_of(ctx), a);
+    if (int rc = check_launch(name)) return rc;
+  }
+  return TTRL_OK;
+}
+
+int ttrl_adamw_moments(ttrl_ctx* ctx, int count, const ttrl_adamw_moment* tensors, const void* m, const void* v,
+                       const float* m_scale, const float* v_scale) {
+  const char* name = "ttrl_adamw_moments";
+  TTRL_REQUIRE(ctx && tensors && m && v && m_scale && v_scale, "%s: null argument", name);
+  TTRL_REQUIRE(count > 0, "%s: no tensors", name);
+  for (int i = 0; i < count; ++i)
+    TTRL_REQUIRE(tensors[i].m && tensors[i].v && tensors[i].n > 0 && tensors[i].n <= (1L << 40) && tensors[i].at >= 0 &&
+                     tensors[i].at % kBlock == 0,
+                 "%s: tensor %d: null, empty, or its moments do not start on a block of %d", name, i, kBlock);
+  for (int from = 0; from < count; from += kTensors) {
+    HeldArgs a{};
+    a.count = std::min(kTensors, count - from);
+    long blocks = 0;
+    for (int i = 0; i < a.count; ++i) {
+      const ttrl_adamw_moment& t = tensors[from + i];
+      a.item[i] = {t.m, t.v, t.at, t.n, int(blocks)};
+      blocks += blocks_of(t.n);
+      TTRL_REQUIRE(blocks <= 0x7fffffffL, "%s: too many elements", name);
+    }
+    a.mc = static_cast<const uint8_t*>(m);
+    a.vc = static_cast<const uint8_t*>(v);
+    a.ms = m_scale;
+    a.vs = v_scale;
+    hipLaunchKernelGGL(k_adamw_held, dim3(unsigned(blocks)), dim3(kThreads), 0, stream_of(ctx), a);
+    if (int rc = check_launch(name)) return rc;
+  }
+  return TTRL_OK;
+}
+
+}  // extern "C"

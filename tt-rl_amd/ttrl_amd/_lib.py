@@ -140,6 +140,41 @@ class AdamSourcesDesc(C.Structure):
     ]
 
 
+class LinearAttentionDesc(C.Structure):
+    """Mirror of ttrl_linear_attention_desc."""
+
+    _fields_ = ([(n, C.c_int) for n in ("T", "B", "H", "kv_heads", "K", "V")]
+                + [(n, C.c_void_p) for n in ("q", "k", "v", "log_decay")]
+                + [("decay_steps", C.c_int), ("done", C.c_void_p), ("scale", C.c_float)]
+                + [(n, C.c_void_p) for n in ("state", "out", "final_state", "saved", "work", "dout", "dfinal", "dq", "dk",
+                                             "dv", "dlog_decay", "dstate")])
+
+
+GATES = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+
+
+class GatedDesc(C.Structure):
+    """Mirror of ttrl_gated_desc."""
+
+    _fields_ = ([(n, C.c_int) for n in ("M", "K", "N", "act")]
+                + [(n, C.c_void_p) for n in ("x", "w_gate", "w_up", "b_gate", "b_up", "g", "u", "h")])
+
+
+ADAMW_COUNTER_BYTES = 24
+
+
+class AdamWTensor(C.Structure):
+    """Mirror of ttrl_adamw_tensor."""
+
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("at", C.c_long), ("n", C.c_long)]
+
+
+class AdamWMoment(C.Structure):
+    """Mirror of ttrl_adamw_moment."""
+
+    _fields_ = [("m", C.c_void_p), ("v", C.c_void_p), ("at", C.c_long), ("n", C.c_long)]
+
+
 class ReplayRing(C.Structure):
     """Mirror of ttrl_replay_ring."""
 
@@ -276,6 +311,16 @@ SIGNATURES = {
     "ttrl_gru_step_backward_fused": ([P, I, I, P, P, P, P, P, P, P, P, P, P, P, P], I),
     "ttrl_gru_step_ragged": ([P, I, I, P, P, P, P, P, P, P, P], I),
     "ttrl_gru_step_backward_ragged": ([P, I, I, P, P, P, P, P, P, P, P, P, P, P, P], I),
+    "ttrl_linear_attention_space": ([C.POINTER(LinearAttentionDesc), C.POINTER(L), C.POINTER(L)], I),
+    "ttrl_linear_attention_forward": ([P, C.POINTER(LinearAttentionDesc)], I),
+    "ttrl_linear_attention_backward": ([P, C.POINTER(LinearAttentionDesc)], I),
+    "ttrl_linear_attention_token": ([P, I, I, I, I, I, P, P, P, P, I, P, F, P, P], I),
+    "ttrl_gated_forward": ([P, C.POINTER(GatedDesc)], I),
+    "ttrl_gated_slopes": ([P, I, I, I, P, P, P, P, P], I),
+    "ttrl_adamw_set_count": ([P, P, I, C.c_double, C.c_double], I),
+    "ttrl_adamw_step": ([P, I, C.POINTER(AdamWTensor), I, P, P, P, P, P, C.c_double, C.c_double, C.c_double, C.c_double,
+                         C.c_double], I),
+    "ttrl_adamw_moments": ([P, I, C.POINTER(AdamWMoment), P, P, P, P], I),
     "ttrl_replay_write": ([P, C.POINTER(ReplayRing), I, P, P, P, P, P, P, P, P, P, P], I),
     "ttrl_replay_lane_sums": ([P, C.POINTER(ReplayRing), P, P, I, I, P, P], I),
     "ttrl_replay_priority_pick": ([P, C.POINTER(ReplayRing), I, P, P, P, P, I, I, P, P, P, P], I),

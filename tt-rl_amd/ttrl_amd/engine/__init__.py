@@ -14,8 +14,8 @@ _LAZY = {
     "register_device_cache": "device", "survey": "device", "probe_profile": "device",
     "DeviceArray": "tensor", "MASTER_DTYPE": "tensor", "ParamArena": "tensor", "copy_in_place": "tensor",
     "copy_tensor_in_place": "tensor", "to_device": "tensor", "to_host": "tensor", "restore_in_place": "tensor",
-    "Tensor": "autograd", "backward": "autograd", "no_grad": "autograd",
-    "Adam": "optim", "Optimizer": "optim", "adam_fused_scalars": "optim",
+    "Tensor": "autograd", "backward": "autograd", "backward_from": "autograd", "no_grad": "autograd",
+    "Adam": "optim", "AdamW": "optim", "Optimizer": "optim", "adam_fused_scalars": "optim",
     "TrainStep": "step", "read_metrics": "step", "MODES": "step",
     "CapturedTrace": "trace", "TraceCaptureError": "trace", "capture": "trace",
     "Linear": "layers", "LayerNorm": "layers", "ReLU": "layers", "Tanh": "layers", "Sequential": "layers",
@@ -31,7 +31,7 @@ __all__ = ["DEFAULT", "EngineConfig", *sorted(_LAZY),
     "clamp", "maximum", "minimum", "matmul", "argmax_dim_detached", "max_dim_detached", "mean_all", "mean_dim",
     "sum_all", "sum_dim", "concat", "reshape", "split", "apply_done_mask", "entropy", "gather_onehot", "huber",
     "log_softmax", "masks", "non_finite_check", "one_hot_device", "one_hot_gather", "one_hot_host",
-    "linear", "dqn_td_loss",
+    "linear", "dqn_td_loss", "gated_linear", "linear_attention", "linear_attention_step",
 ]
 
 

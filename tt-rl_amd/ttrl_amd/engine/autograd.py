@@ -23,7 +23,7 @@ import numpy as np
 
 from ttrl_amd.engine.tensor import DeviceArray, ParamArena, to_device, to_host
 
-__all__ = ["Tensor", "backward", "no_grad", "is_grad_enabled"]
+__all__ = ["Tensor", "backward", "backward_from", "no_grad", "is_grad_enabled"]
 
 _GRAD_ENABLED = True
 
@@ -221,7 +221,6 @@ class Tensor:
                 f"(numel={numel}); there is no `gradient=` kwarg to seed a "
                 "non-scalar backward pass, so reduce to a scalar first."
             )
-        order = _consumers_first(self)
         seed = DeviceArray(self.device, self.shape)
         if self._op in UNIT_SEED_OPS:
             seed.unit = True  # the root's backward reads only the flag: no fill launch
@@ -229,30 +228,36 @@ class Tensor:
             seed.fill(1.0)
         self.grad = seed
         self._grad_owned = True
-        try:
-            for node in order:
-                if node.grad is None:
-                    continue
-                if node._backward_done and node is not self:
-                    raise RuntimeError(
-                        "backward() reached a node whose tape was already "
-                        "consumed by a previous backward() call on a graph "
-                        "sharing this subgraph; reusing a consumed subgraph "
-                        "is not supported (no retain_graph)."
-                    )
-                node._backward(node.grad)
-        finally:
-            for node in order:
-                # Leaves begin the next step's graph: only op nodes are spent.
-                node._backward_done = node._backward_done or bool(node._op)
-                node._backward = _no_backward
-                node._parents = ()
+        _walk((self,))
 
 
-def _consumers_first(root: Tensor) -> list:
-    """Nodes reachable from `root`, each after all of its reachable consumers."""
+def _walk(roots) -> None:
+    """Runs the tape below `roots`, whose gradients are set, and tears it down."""
+    order = _consumers_first(roots)
+    try:
+        for node in order:
+            if node.grad is None:
+                continue
+            if node._backward_done and all(node is not r for r in roots):
+                raise RuntimeError(
+                    "backward() reached a node whose tape was already "
+                    "consumed by a previous backward() call on a graph "
+                    "sharing this subgraph; reusing a consumed subgraph "
+                    "is not supported (no retain_graph)."
+                )
+            node._backward(node.grad)
+    finally:
+        for node in order:
+            # Leaves begin the next step's graph: only op nodes are spent.
+            node._backward_done = node._backward_done or bool(node._op)
+            node._backward = _no_backward
+            node._parents = ()
+
+
+def _consumers_first(roots) -> list:
+    """Nodes reachable from `roots`, each after all of its reachable consumers."""
     pending: dict[int, int] = {}
-    frontier, reached = [root], {id(root)}
+    frontier, reached = list(roots), {id(r) for r in roots}
     while frontier:
         for parent in frontier.pop()._parents:
             key = id(parent)
@@ -260,7 +265,7 @@ def _consumers_first(root: Tensor) -> list:
             if key not in reached:
                 reached.add(key)
                 frontier.append(parent)
-    order, ready = [], [root]
+    order, ready = [], [r for r in roots if id(r) not in pending]  # a root may be below another
     while ready:
         node = ready.pop()
         order.append(node)
@@ -305,6 +310,32 @@ Tensor.__neg__ = _negate
 
 def backward(tensor: Tensor) -> None:
     tensor.backward()
+
+
+def backward_from(seeds) -> None:
+    """Runs the tape from outputs whose gradients come from elsewhere (the
+    rest of a network on another device, a loss formed outside the tape):
+    `seeds` is a sequence of (output, gradient) pairs, a gradient a Tensor or
+    DeviceArray of the output's shape.  As `Tensor.backward`, it runs every
+    closure once and releases the tape."""
+    seeds = [(t, getattr(g, "data", g)) for t, g in seeds]
+    if not seeds:
+        raise ValueError("backward_from: no outputs")
+    for t, g in seeds:
+        if not t.requires_grad or not t._op:
+            raise RuntimeError("backward_from: an output carries no tape (a leaf, a detached node, or built inside "
+                               "no_grad())")
+        if t._backward_done:
+            raise RuntimeError("backward_from: an output's tape was already consumed by a previous pass; build a "
+                               "fresh forward pass instead")
+        if tuple(g.shape) != t.shape:
+            raise ValueError(f"backward_from: an output of shape {t.shape} was given a gradient of shape {tuple(g.shape)}")
+        if g.dtype != np.float32:
+            raise ValueError(f"backward_from: gradients must be float32, got {g.dtype}")
+    for t, g in seeds:
+        t._accumulate(g)
+    roots = {id(t): t for t, _ in seeds}
+    _walk(tuple(roots.values()))
 
 
 def _is_scalar(x) -> bool:

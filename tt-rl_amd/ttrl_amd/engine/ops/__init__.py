@@ -12,6 +12,7 @@ from ttrl_amd.engine.ops.reduce import (
     argmax_dim_detached, max_dim_detached, mean_all, mean_dim, sum_all, sum_dim,
 )
 from ttrl_amd.engine.ops.select import clamp, maximum, minimum
+from ttrl_amd.engine.ops.sequence import gated_linear, linear_attention, linear_attention_step
 from ttrl_amd.engine.ops.shape import concat, reshape, split
 from ttrl_amd.engine.ops.unary import abs_, exp, log, neg, relu, sigmoid, sqrt, square, tanh
 
@@ -28,4 +29,5 @@ __all__ = [
     "one_hot_host",
     "purge_lane_caches", "purge_matmul_caches",
     "linear", "dqn_td_loss",
+    "gated_linear", "linear_attention", "linear_attention_step",
 ]

@@ -29,7 +29,7 @@ from ttrl_amd import _lib
 from ttrl_amd.engine.pending import MAX_SOURCES, MAX_SUMS, settle, settle_sums, take_sources, take_sums
 from ttrl_amd.engine.tensor import DeviceArray, MASTER_DTYPE, arena_of, zeros
 
-__all__ = ["Adam", "Optimizer", "adam_fused_scalars", "adam_multi", "finish_steps"]
+__all__ = ["Adam", "AdamW", "Optimizer", "adam_fused_scalars", "adam_multi", "finish_steps"]
 
 
 def adam_fused_scalars(lr: float, b1: float, b2: float, eps: float, t: int) -> tuple[float, float]:
@@ -375,6 +375,168 @@ class Adam(Optimizer):
         self.steps = steps
         self._arena_t = steps[0] if steps and all(s == steps[0] for s in steps) else -1
         self._counters.upload(np.asarray(self.steps + [max(self._arena_t, 0)], np.int32))
+
+
+#: Elements that share a scale where moments are held in 8 bits; every tensor's
+#: moments start on such a block.
+MOMENT_BLOCK = 64
+
+
+class AdamW(Optimizer):
+    """AdamW over fp32 parameters, updated in place, every tensor in one
+    launch (64 tensors a launch) whether or not they form an arena:
+
+        m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
+        p = (1 - lr wd) p - (lr / bc1) m / (sqrt(v) / sqrt(bc2) + eps).
+
+    `state_bits=8` holds both moments in a byte per element with a scale per
+    block of 64 (4.25 bytes of p's and the moments' 12 less in memory than
+    with 32): m to 1/127 of its block's largest near it and finer below
+    (steps of the square root), v in steps of the fourth root.  The update
+    count lives on the device, so a captured graph with the step replays
+    correctly."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
+        super().__init__(params)
+        if not self.params:
+            raise ValueError("AdamW: params is empty, so there is nothing to optimize")
+        if lr <= 0:
+            raise ValueError(f"AdamW: lr must be > 0, got {lr}")
+        b1, b2 = betas
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"AdamW: betas must be in [0, 1), got {betas}")
+        if eps <= 0:
+            raise ValueError(f"AdamW: eps must be > 0, got {eps}")
+        if weight_decay < 0:
+            raise ValueError(f"AdamW: weight_decay must be >= 0, got {weight_decay}")
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 8 or 32, got {state_bits}")
+        wrong = [i for i, p in enumerate(self.params) if p.data.dtype != MASTER_DTYPE]
+        if wrong:
+            raise ValueError(f"AdamW: parameters must be float32; parameters {wrong} are not")
+        empty = [i for i, p in enumerate(self.params) if p.data.numel == 0]
+        if empty:
+            raise ValueError(f"AdamW: parameters {empty} are empty")
+        if len({id(p) for p in self.params}) != len(self.params):
+            raise ValueError("AdamW: a parameter is listed twice")
+        self.lr = float(lr)
+        self.b1, self.b2 = float(b1), float(b2)
+        self.eps = float(eps)
+        self.weight_decay = float(weight_decay)
+        self.state_bits = int(state_bits)
+        self.t = 0
+        dev = self.device = self.params[0].device
+        self.offsets, n = [], 0
+        for p in self.params:
+            self.offsets.append(n)
+            n += -(-p.data.numel // MOMENT_BLOCK) * MOMENT_BLOCK
+        dtype = np.float32 if state_bits == 32 else np.uint8
+        self._m_flat, self._v_flat = (zeros(dev, (n,), dtype) for _ in range(2))
+        self._scales = () if state_bits == 32 else tuple(zeros(dev, (n // MOMENT_BLOCK,)) for _ in range(2))
+        #: each parameter's moments; in 8 bits their codes (m's signed), `moments()` gives their values
+        self.m, self.v = ([flat.view(at, p.shape) for at, p in zip(self.offsets, self.params)]
+                          for flat in (self._m_flat, self._v_flat))
+        self._counter = DeviceArray(dev, (_lib.ADAMW_COUNTER_BYTES,), np.uint8)
+        self._table, self._table_key = None, None
+        self._set_count()
+
+    def _set_count(self) -> None:
+        self.device.call("ttrl_adamw_set_count", self._counter.vp, int(self.t), self.b1, self.b2)
+
+    def step(self) -> None:
+        """One update of every parameter; each must hold a gradient."""
+        missing = [i for i, p in enumerate(self.params) if p.grad is None]
+        if missing:
+            raise RuntimeError(f"AdamW.step: parameters {missing} hold no gradient for this step")
+        settle(self.params)
+        settle_sums(self.device)
+        key = [p.grad.ptr for p in self.params] + [p.data.ptr for p in self.params]
+        if key != self._table_key:
+            for i, p in enumerate(self.params):
+                if p.grad.numel != p.data.numel or p.grad.dtype != MASTER_DTYPE:
+                    raise ValueError(f"AdamW.step: parameter {i} has shape {p.shape}, its gradient {p.grad.shape} "
+                                     f"({p.grad.dtype})")
+            self._table = (_lib.AdamWTensor * len(self.params))(*[
+                (p.data.ptr, p.grad.ptr, at, p.data.numel) for p, at in zip(self.params, self.offsets)])
+            self._table_key = key
+        ms, vs = (a.vp for a in self._scales) if self._scales else (None, None)
+        self.device.call("ttrl_adamw_step", len(self.params), self._table, self.state_bits, self._m_flat.vp,
+                         self._v_flat.vp, ms, vs, self._counter.vp, self.lr, self.b1, self.b2, self.eps,
+                         self.weight_decay)
+        if not self.device.capturing:
+            self.t += 1
+
+    def _replayed(self, have_grads=None) -> None:
+        """Host bookkeeping after a graph replay that ran one step."""
+        self.t += 1
+
+    def moments(self, out=None):
+        """-> (m, v), lists of float32 arrays of the parameters' shapes: the
+        moments themselves, or the values their 8-bit codes stand for, written
+        to `out` (two such lists) when it is given."""
+        if self.state_bits == 32 and out is None:
+            return list(self.m), list(self.v)
+        if out is None:
+            out = tuple([DeviceArray(self.device, p.shape) for p in self.params] for _ in range(2))
+        for arrays in out:
+            if len(arrays) != len(self.params) or any(a.numel != p.data.numel or a.dtype != np.float32
+                                                      for a, p in zip(arrays, self.params)):
+                raise ValueError("AdamW.moments: out must be two lists of float32 arrays of the parameters' shapes")
+        if self.state_bits == 32:
+            for dst, src in zip(out[0] + out[1], self.m + self.v):
+                dst.copy_from(src.reshape(dst.shape))
+            return tuple(out)
+        table = (_lib.AdamWMoment * len(self.params))(*[
+            (m.ptr, v.ptr, at, p.data.numel) for m, v, at, p in zip(*out, self.offsets, self.params)])
+        self.device.call("ttrl_adamw_moments", len(self.params), table, self._m_flat.vp, self._v_flat.vp,
+                         *(a.vp for a in self._scales))
+        return tuple(out)
+
+    # -- checkpointing -----------------------------------------------------
+
+    def _scale_views(self, which: int) -> list:
+        return [self._scales[which].view(at // MOMENT_BLOCK, (-(-p.data.numel // MOMENT_BLOCK),))
+                for at, p in zip(self.offsets, self.params)]
+
+    def state_dict(self) -> dict:
+        """What a resumed optimizer needs, bit for bit: with 8 bits the codes
+        (m's int8, v's uint8) and each tensor's block scales."""
+        out = {"t": self.t, "lr": self.lr, "betas": (self.b1, self.b2), "eps": self.eps,
+               "weight_decay": self.weight_decay, "state_bits": self.state_bits,
+               "m": [a.numpy() for a in self.m], "v": [a.numpy() for a in self.v]}
+        if self._scales:
+            out["m"] = [a.view(np.int8) for a in out["m"]]
+            out["m_scale"], out["v_scale"] = ([a.numpy() for a in self._scale_views(i)] for i in range(2))
+        return out
+
+    def load_state_dict(self, state: dict, device=None) -> None:
+        bits = int(state.get("state_bits", self.state_bits))
+        if bits != self.state_bits:
+            raise ValueError(f"AdamW.load_state_dict: the checkpoint's moments are in {bits} bits, this optimizer's in "
+                             f"{self.state_bits}")
+        kinds = {"m": (self.m, np.int8), "v": (self.v, np.uint8)}
+        if self._scales:
+            kinds.update({"m_scale": (self._scale_views(0), None), "v_scale": (self._scale_views(1), None)})
+        arrays = {}
+        for key, (buffers, held) in kinds.items():
+            if key not in state or len(state[key]) != len(buffers):
+                raise ValueError(f"AdamW.load_state_dict: expected {len(buffers)} {key} buffers")
+            arrays[key] = [np.asarray(a) for a in state[key]]
+            for i, (a, buf) in enumerate(zip(arrays[key], buffers)):
+                if a.shape != tuple(buf.shape):
+                    raise ValueError(f"AdamW.load_state_dict: {key}[{i}] has shape {a.shape}, expected "
+                                     f"{tuple(buf.shape)}")
+                if self._scales and held is not None and a.dtype != held:
+                    raise ValueError(f"AdamW.load_state_dict: {key}[{i}] holds {a.dtype}, expected {np.dtype(held)} codes")
+        self.t = int(state["t"])
+        self.lr = float(state.get("lr", self.lr))
+        self.b1, self.b2 = (float(x) for x in state.get("betas", (self.b1, self.b2)))
+        self.eps = float(state.get("eps", self.eps))
+        self.weight_decay = float(state.get("weight_decay", self.weight_decay))
+        for key, (buffers, held) in kinds.items():
+            for a, buf in zip(arrays[key], buffers):
+                buf.upload(np.ascontiguousarray(a).view(np.uint8) if self._scales and held is not None else a)
+        self._set_count()
 
 
 def _aligned_copy(x: DeviceArray) -> DeviceArray:
