@@ -842,9 +842,10 @@ int ttrl_gru_step_backward_ragged(ttrl_ctx* ctx, int B, int H, const float* dgh,
  * wanted) [B][H][K][V].  K and V up to 128; T and B may be 0.
  * Nothing that is not finite passes from one episode to another, or to an
  * earlier output.
+ * A step's q, k, v or outputs hold at most 2^24 values.
  * ttrl_linear_attention_space: floats of `saved`, which the forward fills for
- * the backward, and of `work`, which the backward uses; both may then be
- * NULL where 0.  The backward overwrites dq, dk and dv (all required) and
+ * the backward (forward_floats of it where no backward follows), and of
+ * `work`, which the backward uses; each may be NULL where 0.  The backward overwrites dq, dk and dv (all required) and
  * dlog_decay unless NULL; with dlog_decay and dfinal it reads final_state. */
 typedef struct ttrl_linear_attention_desc {
   int T, B, H, kv_heads, K, V;
@@ -868,7 +869,8 @@ typedef struct ttrl_linear_attention_desc {
   float* dlog_decay;
   float* dstate;
 } ttrl_linear_attention_desc;
-int ttrl_linear_attention_space(const ttrl_linear_attention_desc* desc, long* saved_floats, long* work_floats);
+int ttrl_linear_attention_space(const ttrl_linear_attention_desc* desc, long* forward_floats, long* saved_floats,
+                                long* work_floats);
 int ttrl_linear_attention_forward(ttrl_ctx* ctx, const ttrl_linear_attention_desc* desc);
 int ttrl_linear_attention_backward(ttrl_ctx* ctx, const ttrl_linear_attention_desc* desc);
 /* One token of B lanes: state [B][H][K][V] is stepped in place, out [B][H][V];

@@ -33,7 +33,11 @@
 // Where there are few heads and sequences, the sequence is cut into segments
 // that run side by side: a first launch forms what each segment adds to the
 // state, a second joins them in order (start[s + 1] = decay[s] start[s] +
-// added[s]), and the sweeps then start from the joined states.
+// added[s]), and the sweeps then start from the joined states.  Otherwise a
+// sweep runs through and leaves the state at every segment's start.  Either
+// way the backward has S and G at the ends of every segment, and the sum for
+// dL/dg starts again there from <S, G>: over a whole sequence, terms that cancel
+// would leave their rounding behind.
 //
 // Precision: products, sums and states are FP32; the sums of log decays are in
 // double, and each weight is the exponential of a difference of two of them, so
@@ -61,11 +65,12 @@ struct Operand {
 
 struct Sweep {
   Operand x, y, z;
-  float* out;  // (T, B, H, E)
-  Operand dot;  // rows to multiply the output's rows with, or null
-  float* dots;  // [E / 16][B * H][T] partial sums of those products, 16 columns each
+  float* out;          // (T, B, H, E)
+  Operand dot;         // rows to multiply the output's rows with, or null
+  float* dots;         // [E / 16][B * H][T] partial sums of those products, 16 columns each
   const float* start;  // state on entering a segment: [segment][B * H][D * E], or of the first one only
   int start_all;       // one for every segment
+  float* marks;        // where a sweep that runs through leaves the state at the segments' starts, or null
   float* end;          // the last segment's state, [B * H][D * E]
   int end_decay;       // end is the state entering step 0: one more decay
   int sk, se;          // strides of a state's element (d, e)
@@ -80,6 +85,7 @@ struct SweepArgs {
   const float* done;
   int g_rows;  // g is (T, B, H), else (1, H)
   int T, B, H, seg, nseg;
+  int run;        // steps a sweep takes: seg, or T where it runs through
   float* added;   // first launch: [segment][B * H][D * E]
   float* decays;  // first launch: [segment][B * H]
 };
@@ -89,31 +95,54 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, const f32x4& c) {
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
-// One chunk's decays, step i of the chunk in lane i of every wavefront.
-struct Decays {
-  double c;      // sum of the log decays since the chunk's or the episode's start
-  int lo;        // the episode's first step in the chunk, -1: before it
-  float into;    // weight of the state on entering the chunk (0: none)
-  float left;    // weight of the step in the state on leaving it (0: none)
-  float keep;    // weight of the entering state in the leaving one (uniform)
-  int first;     // first step that the leaving state holds (uniform)
-  __device__ __forceinline__ void form(float g, bool reset, int lane) {
-    const int i = lane & 31;
-    const uint32_t starts = uint32_t(__ballot(reset));
-    const uint32_t m = starts & (0xffffffffu >> (31 - i));
-    lo = m ? 31 - __clz(m) : -1;
-    c = reset ? 0.0 : double(g);
-#pragma unroll
-    for (int d = 1; d < kChunk; d <<= 1) {
-      const double t = __shfl_up(c, d, 32);
-      if (i - d >= max(lo, 0)) c += t;
-    }
-    const double ce = __shfl(c, 31, 32);
-    const int le = starts ? 31 - __clz(starts) : -1;
-    first = max(le, 0);
-    into = lo < 0 ? expf(float(c)) : 0.f;
-    left = i >= first ? expf(float(ce - c)) : 0.f;
-    keep = le < 0 ? expf(float(ce)) : 0.f;
+// Memory goes through buffer resources, whose range check replaces branches:
+// an offset past the range loads zeros and drops a store.  A chunk's resource
+// starts at its earliest step and ends with the last step there is, so rows
+// past the end are out of range by themselves; columns past the width get kOut.
+constexpr uint32_t kOut = 0x80000000u;
+constexpr int kFlags = 0x00020000;  // raw 32-bit dwords
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* p, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(a));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(uint32_t(a >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(uint64_t(hi) << 32 | lo), 0,
+                                           __builtin_amdgcn_readfirstlane(bytes), kFlags);
+}
+__device__ __forceinline__ float load1(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+}
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 load4(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+}
+__device__ __forceinline__ void store1(__amdgpu_buffer_rsrc_t r, uint32_t off, float v) {
+  __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, off, 0, 0);
+}
+
+// The sum over a row of 16 lanes, in every one of them.
+__device__ __forceinline__ float row_sum(float x) {
+#define TTRL_ROW_ROR(n) \
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + n, 0xf, 0xf, true))
+  TTRL_ROW_ROR(8);
+  TTRL_ROW_ROR(4);
+  TTRL_ROW_ROR(2);
+  TTRL_ROW_ROR(1);
+#undef TTRL_ROW_ROR
+  return x;
+}
+
+// One head's rows of an operand: chunk c's resource.
+struct Rows {
+  const float* p;  // step 0
+  uint32_t pitch;  // bytes from one step to the next
+  uint32_t width;  // bytes of a row
+  __device__ __forceinline__ Rows(const Operand& o, int B, int b, int h) {
+    p = o.p + (long(b) * o.heads + h / o.share) * o.dim;
+    pitch = uint32_t(B) * uint32_t(o.heads) * uint32_t(o.dim) * 4u;
+    width = uint32_t(o.dim) * 4u;
+  }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk(int t, int n) const {  // n > 0 steps from t on
+    return resource(reinterpret_cast<const char*>(p) + long(t) * pitch, uint32_t(n - 1) * pitch + width);
   }
 };
 
@@ -128,25 +157,60 @@ __device__ __forceinline__ void step_decay(const SweepArgs& a, int t, int b, int
   }
 }
 
-// 32 rows of an operand on their way into LDS.
+// A chunk's decays, formed by one wavefront, row i of the sweep's order in lane i.
+struct Decays {
+  double c[kChunk];    // sum of the log decays since the chunk's or the episode's start
+  float into[kChunk];  // weight of the state on entering the chunk (where lo < 0)
+  float left[kChunk];  // weight of the row in the state on leaving it (from `first` on)
+  int lo[kChunk];      // the episode's first row in the chunk, -1: before it
+  float keep;          // weight of the entering state in the leaving one (0: none)
+  int first;           // first row that the leaving state holds
+  __device__ __forceinline__ void form(float g, bool reset, int lane) {
+    const int i = lane & 31;
+    const uint32_t starts = uint32_t(__ballot(reset));
+    const uint32_t m = starts & (0xffffffffu >> (31 - i));
+    const int l = m ? 31 - __clz(m) : -1;
+    double s = reset ? 0.0 : double(g);
+#pragma unroll
+    for (int d = 1; d < kChunk; d <<= 1) {
+      const double t = __shfl_up(s, d, 32);
+      if (i - d >= max(l, 0)) s += t;
+    }
+    const double e = __shfl(s, 31, 32);
+    const int le = starts ? 31 - __clz(starts) : -1;
+    if (lane < kChunk) {
+      c[i] = s;
+      lo[i] = l;
+      into[i] = expf(float(s));
+      left[i] = expf(float(e - s));
+    }
+    if (lane == 0) {
+      keep = le < 0 ? expf(float(e)) : 0.f;
+      first = max(le, 0);
+    }
+  }
+};
+
+// 32 rows of an operand on their way into LDS, row r of the sweep's order.
 template <int KP, int NT, bool VEC>
-struct Rows {
+struct Stage {
   static constexpr int W = VEC ? 4 : 1, CH = KP / W, PER = (kChunk * CH + NT - 1) / NT;
   static constexpr bool WHOLE = kChunk * CH % NT == 0;
-  float f[PER][W];
-  __device__ __forceinline__ void issue(const Operand& o, long base, long pitch, int s0, int n, int dir, int tid) {
+  uint32_t off[PER];
+  f32x4 v4[VEC ? PER : 1];
+  float v1[VEC ? 1 : PER];
+  __device__ __forceinline__ void init(const Rows& o, int back, int tid) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const int i = tid + u * NT, r = i / CH, c = i % CH * W;
-      const bool in = (WHOLE || r < kChunk) && s0 + r < n && c < o.dim;
-      const float* p = o.p + base + long(dir) * (s0 + r) * pitch + c;
-      if constexpr (VEC) {
-        const f32x4 v = in ? *reinterpret_cast<const f32x4*>(p) : f32x4{0.f, 0.f, 0.f, 0.f};
+      off[u] = (WHOLE || r < kChunk) && uint32_t(c) * 4u < o.width ? uint32_t(back ? kChunk - 1 - r : r) * o.pitch + uint32_t(c) * 4u : kOut;
+    }
+  }
+  __device__ __forceinline__ void issue(__amdgpu_buffer_rsrc_t r) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[u][j] = v[j];
-      } else {
-        f[u][0] = in ? *p : 0.f;
-      }
+    for (int u = 0; u < PER; ++u) {
+      if constexpr (VEC) v4[u] = load4(r, off[u]);
+      else v1[u] = load1(r, off[u]);
     }
   }
   __device__ __forceinline__ void store(float* lds, int tid) const {
@@ -154,91 +218,107 @@ struct Rows {
     for (int u = 0; u < PER; ++u) {
       const int i = tid + u * NT, r = i / CH, c = i % CH * W;
       if (!WHOLE && r >= kChunk) continue;
-      float* d = lds + r * (KP + 4) + c;
-      if constexpr (VEC) *reinterpret_cast<f32x4*>(d) = f32x4{f[u][0], f[u][1], f[u][2], f[u][3]};
-      else *d = f[u][0];
+      if constexpr (VEC) *reinterpret_cast<f32x4*>(lds + r * (KP + 4) + c) = v4[u];
+      else lds[r * (KP + 4) + c] = v1[u];
     }
   }
 };
 
 // LOCAL: the first launch, what a segment adds to the state.
 template <int KP, int NW, bool VEC, bool LOCAL>
-__global__ __launch_bounds__(64 * NW) void k_sweep(SweepArgs a) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 128 && NW == 4 ? 2 : 3))) void k_sweep(SweepArgs a) {
   constexpr int NT = 64 * NW, KB = KP / 16, PX = KP + 4, PP = kChunk + 4;
   __shared__ __attribute__((aligned(16))) float lx[LOCAL ? 1 : 2][LOCAL ? 4 : kChunk * PX];
   __shared__ __attribute__((aligned(16))) float ly[2][kChunk * PX];
   __shared__ __attribute__((aligned(16))) float lp[LOCAL ? 1 : 2][LOCAL ? 4 : kChunk * PP];
+  __shared__ __attribute__((aligned(16))) Decays ld[2];
   const Sweep& w = a.s[blockIdx.z];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
-  const int bh = int(blockIdx.x), b = bh / a.H, h = bh - b * a.H, seg = int(blockIdx.y);
-  const int t0 = seg * a.seg, n = min(a.seg, a.T - t0);
-  const int D = w.x.dim, E = w.z.dim, nkb = (D + 15) / 16;
-  const int dir = w.back ? -1 : 1, tb = w.back ? t0 + n - 1 : t0;  // time of step s: tb + dir * s
-  const int td = w.back ? tb + 1 : tb;                             // of its decay
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int bh = int(blockIdx.x), b = bh / a.H, h = bh - b * a.H, run = int(blockIdx.y);
+  const int t0 = run * a.run, n = min(a.run, a.T - t0), back = w.back;
+  const int D = w.x.dim, E = w.z.dim, nkb = (D + 15) / 16, nch = (n + kChunk - 1) / kChunk;
   const int e = wave * 16 + lr;
+  const bool cols = wave * 16 < E;  // uniform: this wavefront has columns of the state
+  const long BH = long(a.B) * a.H;
 
-  auto base = [&](const Operand& o) { return ((long(tb) * a.B + b) * o.heads + h / o.share) * long(o.dim); };
-  auto pitch = [&](const Operand& o) { return long(a.B) * o.heads * o.dim; };
-  const long bx = LOCAL ? 0 : base(w.x), px = LOCAL ? 0 : pitch(w.x);
-  const long by = base(w.y), py = pitch(w.y), bz = base(w.z), pz = pitch(w.z);
-  const long po = long(a.B) * a.H * E, bo = ((long(tb) * a.B + b) * a.H + h) * long(E);
-
-  f32x4 S[KB];
-  {
-    const float* st = LOCAL ? nullptr : w.start;
-    const bool any = st && (w.start_all || (w.back ? seg + 1 == a.nseg : seg == 0));
-    if (any) st += (w.start_all ? long(seg) * a.B * a.H + bh : long(bh)) * D * E;
-#pragma unroll
-    for (int k = 0; k < KB; ++k)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = k * 16 + 4 * lg + r;
-        S[k][r] = any && d < D && e < E ? st[long(d) * w.sk + long(e) * w.se] : 0.f;
-      }
-  }
-
-  Rows<KP, NT, VEC> rx, ry;
-  float zn[2][4];
-  float gn;
-  bool fn;
-  auto fetch = [&](int s0) {
-    if constexpr (!LOCAL) rx.issue(w.x, bx, px, s0, n, dir, tid);
-    ry.issue(w.y, by, py, s0, n, dir, tid);
+  const Rows rx(w.x, a.B, b, h), ry(w.y, a.B, b, h), rz(w.z, a.B, b, h);
+  const Rows ro(Operand{w.out, a.H, E, 1}, a.B, b, h);
+  Stage<KP, NT, VEC> sx, sy;
+  if constexpr (!LOCAL) sx.init(rx, back, tid);
+  sy.init(ry, back, tid);
+  // Rows jb * 16 + 4 * lg + r of the sweep's order, this lane's column.
+  auto offset = [&](uint32_t pitch, int jb, int r) {
+    const int at = back ? (12 - 4 * lg) + (3 - r) + 16 * (1 - jb) : 4 * lg + r + 16 * jb;
+    return e < E ? uint32_t(at) * pitch + uint32_t(e) * 4u : kOut;
+  };
+  auto element = [&](int k, int r) {
+    const int d = k * 16 + 4 * lg + r;
+    return d < D && e < E ? uint32_t(d * w.sk + e * w.se) * 4u : kOut;
+  };
+  float zn[2][4], gn = 0.f;
+  bool fn = false;
+  auto fetch = [&](int c) {  // chunk c
+    const int t = t0 + c * kChunk, m = n - c * kChunk;
+    if constexpr (!LOCAL) sx.issue(rx.chunk(t, min(m, kChunk)));
+    sy.issue(ry.chunk(t, min(m, kChunk)));
+    const __amdgpu_buffer_rsrc_t r2 = rz.chunk(t, min(m, kChunk));
 #pragma unroll
     for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int s = s0 + jb * 16 + 4 * lg + r;
-        zn[jb][r] = s < n && e < E ? w.z.p[bz + long(dir) * s * pz + e] : 0.f;
-      }
-    const int s = s0 + (lane & 31);
-    gn = 0.f;
-    fn = false;
-    if (s < n) step_decay(a, td + dir * s, b, h, gn, fn);
+      for (int r = 0; r < 4; ++r) zn[jb][r] = load1(r2, offset(rz.pitch, jb, r));
+    if (wave == 0) {  // backwards a step's decay is the one of the step after it
+      const int i = lane & 31, s = back ? kChunk - i : i;
+      step_decay(a, t + s, b, h, gn, fn);
+      if (s >= m + back) gn = 0.f, fn = false;
+    }
   };
-  fetch(0);
+  f32x4 S[KB];
+  fetch(back ? nch - 1 : 0);
+  {
+    const bool any = !LOCAL && w.start && (w.start_all || (back ? t0 + n == a.T : t0 == 0));
+    const __amdgpu_buffer_rsrc_t r0 =
+        resource(any ? w.start + (w.start_all ? run * BH + bh : long(bh)) * D * E : w.y.p, any ? uint32_t(D) * E * 4u : 0);
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[k][r] = load1(r0, element(k, r));
+  }
+  auto leave = [&](float* to, float scale, bool none) {
+    const __amdgpu_buffer_rsrc_t r0 = resource(to, uint32_t(D) * E * 4u);
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) store1(r0, element(k, r), none ? 0.f : S[k][r] * scale);
+  };
+
   float total = 1.f;
-  int buf = 0;
-  for (int s0 = 0; s0 < n; s0 += kChunk, buf ^= 1) {
+  for (int i = 0; i < nch; ++i) {
+    const int c = back ? nch - 1 - i : i, buf = i & 1;
     float* X = lx[LOCAL ? 0 : buf];
     float* Y = ly[buf];
     float* P = lp[LOCAL ? 0 : buf];
-    if constexpr (!LOCAL) rx.store(X, tid);
-    ry.store(Y, tid);
+    Decays& dc = ld[buf];
+    if constexpr (!LOCAL) {
+      sx.store(X, tid);
+      if (w.marks && (back ? i == 0 || (c + 1) * kChunk % a.seg == 0 : c * kChunk % a.seg == 0))
+        leave(w.marks + (c * kChunk / a.seg * BH + bh) * D * E, 1.f, false);
+    }
+    sy.store(Y, tid);
     float z[2][4];
 #pragma unroll
     for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) z[jb][r] = zn[jb][r];
-    Decays dc;
-    dc.form(gn, fn, lane);
-    if (s0 + kChunk < n) fetch(s0 + kChunk);
+    if (wave == 0) dc.form(gn, fn, lane);
+    if (i + 1 < nch) fetch(back ? c - 1 : c + 1);
     __syncthreads();
 
     if constexpr (!LOCAL) {
-      // Weights of the chunk's own steps: the three 16 x 16 blocks that have any.
-      for (int f = wave; f < 3; f += NW) {
-        const int ri = f > 0, cj = f > 1;
+      // Weights of the chunk's own rows: the three 16 x 16 blocks that have
+      // any, by the last wavefronts (the ones without columns, if there are).
+      for (int f = NW - 1 - wave; f < 3; f += NW) {
+        const int ri = f > 0, cj = f > 1, j = cj * 16 + lr;
         f32x4 p = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < KB; ++k) {
@@ -248,146 +328,152 @@ __global__ __launch_bounds__(64 * NW) void k_sweep(SweepArgs a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) p = mfma4(xa[r], yb[r], p);
         }
-        const int j = cj * 16 + lr;
-        const double cjv = __shfl(dc.c, j, 32);
+        const double cj0 = dc.c[j];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int i = ri * 16 + 4 * lg + r;
-          const double ci = __shfl(dc.c, i, 32);
-          const int lo = __shfl(dc.lo, i, 32);
-          P[i * PP + j] = j <= i && j >= lo ? p[r] * (expf(float(ci - cjv)) * w.alpha_out * w.alpha_pair) : 0.f;
+          const int row = ri * 16 + 4 * lg + r;
+          const float wt = expf(float(dc.c[row] - cj0)) * (w.alpha_out * w.alpha_pair);
+          P[row * PP + j] = j <= row && j >= dc.lo[row] ? p[r] * wt : 0.f;
         }
       }
       // What the entering state gives each row.
       f32x4 o[2];
 #pragma unroll
       for (int f = 0; f < 2; ++f) o[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (cols) {
 #pragma unroll
-      for (int k = 0; k < KB; ++k) {
-        if (k >= nkb) break;
+        for (int k = 0; k < KB; ++k) {
+          if (k >= nkb) break;
+          f32x4 xa[2];
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const f32x4 xa = *reinterpret_cast<const f32x4*>(X + (f * 16 + lr) * PX + k * 16 + 4 * lg);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[f] = mfma4(xa[r], S[k][r], o[f]);
-        }
-      }
-#pragma unroll
-      for (int f = 0; f < 2; ++f)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = f * 16 + 4 * lg + r;
-          const float in = __shfl(dc.into, i, 32);
-          const int lo = __shfl(dc.lo, i, 32);
-          o[f][r] = lo < 0 ? o[f][r] * (in * w.alpha_out) : 0.f;
-        }
-      __syncthreads();
-      bool odd = false;
-#pragma unroll
-      for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) odd = odd || !finite(z[jb][r]);
-      if (!__any(odd)) {
-#pragma unroll
-        for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-          for (int f = jb; f < 2; ++f) {
-            const f32x4 pa = *reinterpret_cast<const f32x4*>(P + (f * 16 + lr) * PP + jb * 16 + 4 * lg);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[f] = mfma4(pa[r], z[jb][r], o[f]);
-          }
-      } else {
-#pragma unroll
-        for (int jb = 0; jb < 2; ++jb)
+          for (int f = 0; f < 2; ++f) xa[f] = *reinterpret_cast<const f32x4*>(X + (f * 16 + lr) * PX + k * 16 + 4 * lg);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-#pragma unroll 1
-            for (int m = 0; m < 4; ++m) {
-              const int j = jb * 16 + 4 * m + r;
-              const float zj = __shfl(z[jb][r], lr + 16 * m, 64);
 #pragma unroll
-              for (int f = jb; f < 2; ++f)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const int i = f * 16 + 4 * lg + q, lo = __shfl(dc.lo, i, 32);
-                  if (j <= i && j >= lo) o[f][q] += P[i * PP + j] * zj;
-                }
-            }
-      }
-#pragma unroll
-      for (int f = 0; f < 2; ++f)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int s = s0 + f * 16 + 4 * lg + r;
-          if (s < n && e < E) w.out[bo + long(dir) * s * po + e] = o[f][r];
+            for (int f = 0; f < 2; ++f) o[f] = mfma4(xa[f][r], S[k][r], o[f]);
         }
-      if (w.dot.p) {
-        const long bd = base(w.dot), pd = pitch(w.dot);
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int s = s0 + f * 16 + 4 * lg + r;
-            float d = s < n && e < E ? w.dot.p[bd + long(dir) * s * pd + e] * o[f][r] : 0.f;
-#pragma unroll
-            for (int m = 1; m < 16; m <<= 1) d += __shfl_xor(d, m, 64);
-            if (lr == 0 && s < n && wave * 16 < E)
-              w.dots[(long(wave) * a.B * a.H + bh) * a.T + tb + dir * s] = d;
+            const int row = f * 16 + 4 * lg + r;
+            o[f][r] = dc.lo[row] < 0 ? o[f][r] * (dc.into[row] * w.alpha_out) : 0.f;
           }
+      }
+      __syncthreads();
+      if (cols) {
+        bool odd = false;
+#pragma unroll
+        for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) odd = odd || !finite(z[jb][r]);
+        if (!__any(odd)) {
+#pragma unroll
+          for (int jb = 0; jb < 2; ++jb) {
+            f32x4 pa[2];
+#pragma unroll
+            for (int f = jb; f < 2; ++f) pa[f] = *reinterpret_cast<const f32x4*>(P + (f * 16 + lr) * PP + jb * 16 + 4 * lg);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int f = jb; f < 2; ++f) o[f] = mfma4(pa[f][r], z[jb][r], o[f]);
+          }
+        } else {
+#pragma unroll
+          for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll 1
+              for (int m = 0; m < 4; ++m) {
+                const int j = jb * 16 + 4 * m + r;
+                const float zj = __shfl(z[jb][r], lr + 16 * m, 64);
+#pragma unroll
+                for (int f = jb; f < 2; ++f)
+#pragma unroll
+                  for (int q = 0; q < 4; ++q) {
+                    const int row = f * 16 + 4 * lg + q;
+                    if (j <= row && j >= dc.lo[row]) o[f][q] += P[row * PP + j] * zj;
+                  }
+              }
+        }
+        const int t = t0 + c * kChunk, m = min(n - c * kChunk, kChunk);
+        const __amdgpu_buffer_rsrc_t r2 = ro.chunk(t, m);
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) store1(r2, offset(ro.pitch, f, r), o[f][r]);
+        if (w.dot.p) {
+          const Rows rd(w.dot, a.B, b, h);
+          const __amdgpu_buffer_rsrc_t r3 = rd.chunk(t, m);
+          float* to = w.dots + (long(wave) * BH + bh) * a.T + t;
+          float d[2][4];
+#pragma unroll
+          for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d[f][r] = load1(r3, offset(rd.pitch, f, r)) * o[f][r];
+#pragma unroll
+          for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int row = f * 16 + 4 * lg + r, s = back ? kChunk - 1 - row : row;
+              const float sum = row_sum(e < E ? d[f][r] : 0.f);
+              if (lr == 0 && s < m) to[s] = sum;
+            }
+        }
       }
     }
 
     // The state on leaving the chunk.
+    const float keep = dc.keep;
+    const int first = __builtin_amdgcn_readfirstlane(dc.first);
+    total *= keep;
+    if (cols) {
 #pragma unroll
-    for (int k = 0; k < KB; ++k)
+      for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) S[k][r] = dc.first > 0 || dc.keep == 0.f ? 0.f : S[k][r] * dc.keep;
-    total *= dc.keep;
-#pragma unroll
-    for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = jb * 16 + 4 * lg + r;
-        const float lf = __shfl(dc.left, j, 32);
-        z[jb][r] = j >= dc.first ? z[jb][r] * (lf * w.alpha_pair) : 0.f;
-      }
-#pragma unroll
-    for (int k = 0; k < KB; ++k) {
-      if (k >= nkb) break;
+        for (int r = 0; r < 4; ++r) S[k][r] = keep == 0.f ? 0.f : S[k][r] * keep;
 #pragma unroll
       for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = jb * 16 + 4 * lg + r;
-          float y = Y[j * PX + k * 16 + lr];
-          if (dc.first > 0) y = j >= dc.first ? y : 0.f;
-          S[k] = mfma4(y, z[jb][r], S[k]);
+          z[jb][r] = j >= first ? z[jb][r] * (dc.left[j] * w.alpha_pair) : 0.f;
         }
+      if (first == 0) {
+#pragma unroll
+        for (int k = 0; k < KB; ++k) {
+          if (k >= nkb) break;
+#pragma unroll
+          for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              S[k] = mfma4(Y[(jb * 16 + 4 * lg + r) * PX + k * 16 + lr], z[jb][r], S[k]);
+        }
+      } else {  // rows before `first` are another episode's
+#pragma unroll
+        for (int k = 0; k < KB; ++k) {
+          if (k >= nkb) break;
+#pragma unroll
+          for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int j = jb * 16 + 4 * lg + r;
+              const float y = Y[j * PX + k * 16 + lr];
+              S[k] = mfma4(j >= first ? y : 0.f, z[jb][r], S[k]);
+            }
+        }
+      }
     }
   }
 
-  float* end = nullptr;
-  float scale = 1.f;
-  bool none = false;
   if constexpr (LOCAL) {
-    end = a.added + (long(seg) * a.B * a.H + bh) * D * E;
-    if (tid == 0) a.decays[long(seg) * a.B * a.H + bh] = total;
-  } else if (w.end && (w.back ? seg == 0 : seg + 1 == a.nseg)) {
-    end = w.end + long(bh) * D * E;
-    if (w.end_decay) {
-      float g;
-      step_decay(a, 0, b, h, g, none);
-      scale = expf(g);
-    }
-  }
-  if (end) {
-#pragma unroll
-    for (int k = 0; k < KB; ++k)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = k * 16 + 4 * lg + r;
-        if (d < D && e < E) end[long(d) * w.sk + long(e) * w.se] = none ? 0.f : S[k][r] * scale;
-      }
+    leave(a.added + (run * BH + bh) * D * E, 1.f, false);
+    if (tid == 0) a.decays[run * BH + bh] = total;
+  } else if (w.end && (back ? t0 == 0 : t0 + n == a.T)) {
+    float g = 0.f;
+    bool none = false;
+    if (w.end_decay) step_decay(a, 0, b, h, g, none);
+    leave(w.end + long(bh) * D * E, expf(g), none);
   }
 }
 
@@ -409,73 +495,74 @@ __global__ __launch_bounds__(kJoinThreads) void k_join(float* __restrict__ added
   }
 }
 
-// cross[s][bh] = <state before, gradient state after> at the end of segment s:
-// the gradient of the log decays up to there from what lies beyond.
-__global__ __launch_bounds__(kJoinThreads) void k_cross(SweepArgs a, const float* __restrict__ states,
-                                                        const float* __restrict__ grads,
-                                                        const float* __restrict__ final_state,
-                                                        const float* __restrict__ final_grad, int DE,
-                                                        float* __restrict__ cross) {
-  __shared__ float red[kJoinThreads / 64];
+// dL/dg of one head's segment.  What lies beyond the segment comes in as
+// <state before, gradient state after> at its end; inside, X of a step is the
+// sum of the rows' products from it to the end of its episode.
+constexpr int kGradThreads = 256, kMark = kGradThreads;  // a segment's steps at most
+__global__ __launch_bounds__(kGradThreads) void k_decay_grad(SweepArgs a, const float* __restrict__ states,
+                                                             const float* __restrict__ grads,
+                                                             const float* __restrict__ final_state,
+                                                             const float* __restrict__ final_grad, int DE,
+                                                             const float* __restrict__ qd, const float* __restrict__ kd,
+                                                             int parts, float* __restrict__ dg,
+                                                             double* __restrict__ sums) {
+  constexpr int NWV = kGradThreads / 64;
+  __shared__ float red[NWV];
+  __shared__ double ends[NWV], part[NWV];
+  __shared__ int any[NWV];
   const long BH = long(a.B) * a.H, bh = blockIdx.x;
-  const int s = int(blockIdx.y), b = int(bh / a.H), h = int(bh - long(b) * a.H);
-  const bool last = s + 1 == a.nseg;
-  const float* x = last ? final_state + bh * DE : states + ((s + 1) * BH + bh) * DE;
-  const float* y = last ? final_grad : grads + s * BH * DE;
-  float d = 0.f;
-  if (y) {
-    y += bh * DE;
-    for (int i = threadIdx.x; i < DE; i += kJoinThreads) d += x[i] * y[i];
-  }
-  d = block_sum<kJoinThreads>(d, red);
-  if (threadIdx.x) return;
-  float g;
-  bool reset;
-  step_decay(a, (s + 1) * a.seg, b, h, g, reset);  // past the last step: no decay
-  cross[s * BH + bh] = reset || !y ? 0.f : (last ? d : d * expf(g));
-}
-
-// dL/dg from the rows' products: a wavefront walks one head's segment back.
-__global__ __launch_bounds__(64) void k_decay_grad(SweepArgs a, const float* __restrict__ qd, int nq,
-                                                   const float* __restrict__ kd, int nk,
-                                                   const float* __restrict__ cross, float* __restrict__ dg,
-                                                   double* __restrict__ sums) {
-  const long BH = long(a.B) * a.H, bh = blockIdx.x;
-  const int s = int(blockIdx.y), lane = threadIdx.x, b = int(bh / a.H), h = int(bh - long(b) * a.H);
-  const int t0 = s * a.seg, n = min(a.seg, a.T - t0);
-  double carry = cross ? double(cross[s * BH + bh]) : 0.0, sum = 0.0;
-  for (int e = n; e > 0; e -= 64) {
-    const int t = t0 + e - 1 - lane;  // lane 0 the latest step
-    const bool in = lane < e;
-    double x = 0.0;
-    float g = 0.f;
-    bool reset = false;
-    if (in) {
-      for (int i = 0; i < nq; ++i) x += double(qd[(i * BH + bh) * a.T + t]);
-      for (int i = 0; i < nk; ++i) x -= double(kd[(i * BH + bh) * a.T + t]);
-      step_decay(a, t, b, h, g, reset);
+  const int s = int(blockIdx.y), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = int(bh / a.H), h = int(bh - long(b) * a.H);
+  const int t0 = s * a.seg, n = min(a.seg, a.T - t0), t = t0 + n - 1 - tid;  // thread 0 the latest step
+  const bool in = tid < n, last = s + 1 == a.nseg;
+  double x = 0.0;
+  float g = 0.f;
+  bool reset = false;
+  if (in) {
+    float v[2][kMaxHead / 16];
+    for (int i = 0; i < parts; ++i) {
+      v[0][i] = qd[(i * BH + bh) * a.T + t];
+      v[1][i] = kd[(i * BH + bh) * a.T + t];
     }
-    // X of a step sums the terms from it to the end of its episode: those of
-    // the lanes before it, down to the one after the last start among them.
-    const uint64_t starts = __ballot(reset);
-    const uint64_t before = lane ? starts & (~0ull >> (64 - lane)) : 0ull;
-    const int lo = before ? 64 - __clzll(before) : 0;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double y = __shfl_up(x, d, 64);
-      if (lane - d >= lo) x += y;
-    }
-    if (!before) x += carry;
-    if (reset) x = 0.0;
-    if (in && dg) dg[(long(t) * a.B + b) * a.H + h] = float(x);
-    if (in) sum += x;
-    carry = __shfl(x, min(e, 64) - 1, 64);
+    step_decay(a, t, b, h, g, reset);
+    for (int i = 0; i < parts; ++i) x += double(v[0][i]) - double(v[1][i]);
   }
-  if (sums) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m, 64);
-    if (lane == 0) sums[s * BH + bh] = sum;
+  const float* sx = last ? final_state + bh * DE : states + ((s + 1) * BH + bh) * DE;
+  const float* sy = last ? (final_grad ? final_grad + bh * DE : nullptr) : grads + (s * BH + bh) * DE;
+  double carry = 0.0;
+  if (sy) {  // uniform
+    float d = 0.f;
+    for (int i = tid; i < DE; i += kGradThreads) d += sx[i] * sy[i];
+    d = block_sum<kGradThreads>(d, red);
+    float ge;
+    bool re;
+    step_decay(a, t0 + n, b, h, ge, re);  // past the last step: no decay
+    carry = re ? 0.0 : double(d) * double(expf(ge));
   }
+  const uint64_t starts = __ballot(reset);
+  const uint64_t before = lane ? starts & (~0ull >> (64 - lane)) : 0ull;
+  const int lo = before ? 64 - __clzll(before) : 0;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double y = __shfl_up(x, d, 64);
+    if (lane - d >= lo) x += y;
+  }
+  if (lane == 63) {
+    ends[wave] = reset ? 0.0 : x;
+    any[wave] = starts != 0;
+  }
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) carry = any[i] ? ends[i] : ends[i] + carry;
+  if (!before) x += carry;
+  if (reset) x = 0.0;
+  if (in && dg) dg[(long(t) * a.B + b) * a.H + h] = float(x);
+  if (!sums) return;
+  double sum = in ? x : 0.0;
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m, 64);
+  if (lane == 0) part[wave] = sum;
+  __syncthreads();
+  if (tid == 0) sums[s * BH + bh] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 // The gradient of a decay that all steps share: the sums of its head, in order.
@@ -577,14 +664,14 @@ int launch_sweeps(ttrl_ctx* ctx, const SweepArgs& a, int count, const char* name
     E = std::max(E, a.s[i].z.dim);
     vec = vec && wide(a.s[i].y) && (LOCAL || wide(a.s[i].x));
   }
-  const dim3 grid(unsigned(a.B) * unsigned(a.H), unsigned(a.nseg), unsigned(count));
+  const dim3 grid(unsigned(a.B) * unsigned(a.H), unsigned((a.T + a.run - 1) / a.run), unsigned(count));
   auto go = [&](auto kp, auto nw) {
     constexpr int KP = decltype(kp)::value, NW = decltype(nw)::value;
     if (vec) hipLaunchKernelGGL((k_sweep<KP, NW, true, LOCAL>), grid, dim3(64 * NW), 0, stream_of(ctx), a);
     else hipLaunchKernelGGL((k_sweep<KP, NW, false, LOCAL>), grid, dim3(64 * NW), 0, stream_of(ctx), a);
   };
   auto width = [&](auto kp) {
-    if (E <= 32) go(kp, std::integral_constant<int, 2>{});
+    if (decltype(kp)::value <= 64 && E <= 32) go(kp, std::integral_constant<int, decltype(kp)::value <= 64 ? 2 : 4>{});
     else if (E <= 64) go(kp, std::integral_constant<int, 4>{});
     else go(kp, std::integral_constant<int, 8>{});
   };
@@ -594,21 +681,23 @@ int launch_sweeps(ttrl_ctx* ctx, const SweepArgs& a, int count, const char* name
   return check_launch(name);
 }
 
-// Segments of a sequence: enough workgroups for the 256 compute units, and
-// whole chunks.
+// Segments of whole chunks, kMark steps at most, and whether they run side by
+// side (`cut`): where heads and sequences alone do not fill the compute units.
 struct Plan {
   int seg, nseg;
+  bool cut;
 };
 Plan plan_of(int T, long BH) {
-  const long want = std::max(1L, (1024 + BH - 1) / std::max(1L, BH));
   const long chunks = std::max(1L, long(T + kChunk - 1) / kChunk);
-  const long per = (chunks + want - 1) / want;
+  const long want = std::max(1L, (1024 + BH - 1) / std::max(1L, BH));
+  const bool cut = BH < 256 && chunks > 1;
+  const long per = cut ? std::min(long(kMark / kChunk), (chunks + want - 1) / want) : kMark / kChunk;
   const int seg = int(per * kChunk);
-  return {seg, std::max(1, (T + seg - 1) / seg)};
+  return {seg, std::max(1, (T + seg - 1) / seg), cut && T > seg};
 }
 
 struct Space {  // floats of the caller's buffers, in order
-  long states, decays, grads, gdecays, cross, qdots, kdots, dk, dv, sums;
+  long states, decays, grads, gdecays, qdots, kdots, dk, dv, sums;
 };
 
 int check_desc(const ttrl_linear_attention_desc* d, const char* name) {
@@ -619,6 +708,8 @@ int check_desc(const ttrl_linear_attention_desc* d, const char* name) {
                "%s: head widths of 1 to %d are supported, got K=%d, V=%d", name, kMaxHead, d->K, d->V);
   TTRL_REQUIRE(long(d->B) * d->H <= 0x7fffffffL / 2, "%s: %d sequences of %d heads are too many", name, d->B, d->H);
   TTRL_REQUIRE(plan_of(d->T, long(d->B) * d->H).nseg <= 65535, "%s: %d steps are too many", name, d->T);
+  TTRL_REQUIRE(long(d->B) * d->H * std::max(d->K, d->V) <= 1L << 24,
+               "%s: %d sequences of %d heads are more than 2^24 values a step", name, d->B, d->H);
   return TTRL_OK;
 }
 
@@ -633,6 +724,7 @@ SweepArgs args_of(const ttrl_linear_attention_desc* d) {
   a.H = d->H;
   a.seg = p.seg;
   a.nseg = p.nseg;
+  a.run = p.cut ? p.seg : d->T;
   return a;
 }
 
@@ -645,7 +737,6 @@ Space space_of(const ttrl_linear_attention_desc* d, int nseg) {
   s.decays = S > 1 ? even(S * BH) : 0;
   s.grads = s.states;
   s.gdecays = s.decays;
-  s.cross = even(S * BH);
   s.qdots = even(long((d->K + 15) / 16) * BH * d->T);
   s.kdots = s.qdots;
   s.dk = shared ? even(rows * d->H * d->K) : 0;
@@ -661,12 +752,15 @@ using namespace ttrl;
 
 extern "C" {
 
-int ttrl_linear_attention_space(const ttrl_linear_attention_desc* d, long* saved_floats, long* work_floats) {
+int ttrl_linear_attention_space(const ttrl_linear_attention_desc* d, long* forward_floats, long* saved_floats,
+                                long* work_floats) {
   if (int rc = check_desc(d, "ttrl_linear_attention_space")) return rc;
-  TTRL_REQUIRE(saved_floats && work_floats, "ttrl_linear_attention_space: null output");
-  const Space s = space_of(d, plan_of(d->T, long(d->B) * d->H).nseg);
+  TTRL_REQUIRE(forward_floats && saved_floats && work_floats, "ttrl_linear_attention_space: null output");
+  const Plan p = plan_of(d->T, long(d->B) * d->H);
+  const Space s = space_of(d, p.nseg);
   *saved_floats = s.states + s.decays;
-  *work_floats = s.grads + s.gdecays + s.cross + s.qdots + s.kdots + s.dk + s.dv + s.sums;
+  *forward_floats = p.cut ? *saved_floats : 0;
+  *work_floats = s.grads + s.gdecays + s.qdots + s.kdots + s.dk + s.dv + s.sums;
   return TTRL_OK;
 }
 
@@ -695,7 +789,9 @@ int ttrl_linear_attention_forward(ttrl_ctx* ctx, const ttrl_linear_attention_des
   s.se = 1;
   s.alpha_out = d->scale;
   s.alpha_pair = 1.f;
-  if (a.nseg > 1) {
+  if (a.run == a.T) {
+    s.marks = a.nseg > 1 ? d->saved : nullptr;
+  } else {
     TTRL_REQUIRE(d->saved, "%s: null saved states", name);
     const Space sp = space_of(d, a.nseg);
     a.added = d->saved;
@@ -733,12 +829,12 @@ int ttrl_linear_attention_backward(ttrl_ctx* ctx, const ttrl_linear_attention_de
     at += n;
     return p;
   };
-  float *grads = take(sp.grads), *gdecays = take(sp.gdecays), *cross = take(sp.cross), *qdots = take(sp.qdots),
+  float *grads = take(sp.grads), *gdecays = take(sp.gdecays), *qdots = take(sp.qdots),
         *kdots = take(sp.kdots), *dkh = take(sp.dk), *dvh = take(sp.dv), *sums = take(sp.sums);
   const Operand q{d->q, d->H, d->K, 1}, k{d->k, d->kv_heads, d->K, share}, v{d->v, d->kv_heads, d->V, share},
       go{d->dout, d->H, d->V, 1};
-  const bool cut = a.nseg > 1;
-  TTRL_REQUIRE(!cut || d->saved, "%s: null saved states", name);
+  const bool cut = a.run < a.T;
+  TTRL_REQUIRE(a.nseg == 1 || d->saved, "%s: null saved states", name);
 
   Sweep dv{};  // state G, (K, V)
   dv.x = k;
@@ -763,6 +859,8 @@ int ttrl_linear_attention_backward(ttrl_ctx* ctx, const ttrl_linear_attention_de
     if (int rc = check_launch(name)) return rc;
     dv.start = grads;
     dv.start_all = 1;
+  } else if (a.nseg > 1 && d->dlog_decay) {
+    dv.marks = grads;
   }
   Sweep dk = dv;  // state G^T, (V, K)
   dk.x = v;
@@ -770,6 +868,7 @@ int ttrl_linear_attention_backward(ttrl_ctx* ctx, const ttrl_linear_attention_de
   dk.z = q;
   dk.out = share > 1 ? dkh : d->dk;
   dk.end = nullptr;
+  dk.marks = nullptr;
   dk.sk = 1;
   dk.se = d->V;
   Sweep dq{};  // state S^T, (V, K)
@@ -795,18 +894,11 @@ int ttrl_linear_attention_backward(ttrl_ctx* ctx, const ttrl_linear_attention_de
   if (int rc = launch_sweeps<false>(ctx, a, 3, name)) return rc;
 
   if (d->dlog_decay) {
-    const dim3 each(unsigned(BH), unsigned(a.nseg));
-    const bool crossing = cut || d->dfinal;
-    if (crossing) {
-      TTRL_REQUIRE(!d->dfinal || d->final_state, "%s: the final state's gradient needs the final state", name);
-      hipLaunchKernelGGL(k_cross, each, dim3(kJoinThreads), 0, stream_of(ctx), a, d->saved, grads, d->final_state,
-                         d->dfinal, int(DE), cross);
-      if (int rc = check_launch(name)) return rc;
-    }
+    TTRL_REQUIRE(!d->dfinal || d->final_state, "%s: the final state's gradient needs the final state", name);
     double* total = d->decay_steps ? nullptr : reinterpret_cast<double*>(sums);
-    const int parts = (d->K + 15) / 16;
-    hipLaunchKernelGGL(k_decay_grad, each, dim3(64), 0, stream_of(ctx), a, qdots, parts, kdots, parts,
-                       crossing ? cross : nullptr, d->decay_steps ? d->dlog_decay : nullptr, total);
+    hipLaunchKernelGGL(k_decay_grad, dim3(unsigned(BH), unsigned(a.nseg)), dim3(kGradThreads), 0, stream_of(ctx), a,
+                       d->saved, grads, d->final_state, d->dfinal, int(DE), qdots, kdots, (d->K + 15) / 16,
+                       d->decay_steps ? d->dlog_decay : nullptr, total);
     if (int rc = check_launch(name)) return rc;
     if (total) {
       hipLaunchKernelGGL(k_decay_total, dim3(unsigned(d->H)), dim3(64), 0, stream_of(ctx), total, d->H,

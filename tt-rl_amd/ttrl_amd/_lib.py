@@ -311,7 +311,7 @@ SIGNATURES = {
     "ttrl_gru_step_backward_fused": ([P, I, I, P, P, P, P, P, P, P, P, P, P, P, P], I),
     "ttrl_gru_step_ragged": ([P, I, I, P, P, P, P, P, P, P, P], I),
     "ttrl_gru_step_backward_ragged": ([P, I, I, P, P, P, P, P, P, P, P, P, P, P, P], I),
-    "ttrl_linear_attention_space": ([C.POINTER(LinearAttentionDesc), C.POINTER(L), C.POINTER(L)], I),
+    "ttrl_linear_attention_space": ([C.POINTER(LinearAttentionDesc), C.POINTER(L), C.POINTER(L), C.POINTER(L)], I),
     "ttrl_linear_attention_forward": ([P, C.POINTER(LinearAttentionDesc)], I),
     "ttrl_linear_attention_backward": ([P, C.POINTER(LinearAttentionDesc)], I),
     "ttrl_linear_attention_token": ([P, I, I, I, I, I, P, P, P, P, I, P, F, P, P], I),

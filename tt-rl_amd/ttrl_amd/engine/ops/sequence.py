@@ -103,14 +103,17 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: 
     d.q, d.k, d.v, d.log_decay, d.decay_steps = q.data.ptr, k.data.ptr, v.data.ptr, log_decay.data.ptr, int(steps)
     d.done, d.state = _p(done), _p(state)
     d.scale = 1.0 / math.sqrt(width) if scale is None else float(scale)
-    saved_n, work_n = C.c_long(), C.c_long()
-    _lib.check(_lib.lib().ttrl_linear_attention_space(C.byref(d), C.byref(saved_n), C.byref(work_n)), "linear_attention")
+    space = [C.c_long() for _ in range(3)]
+    _lib.check(_lib.lib().ttrl_linear_attention_space(C.byref(d), *(C.byref(n) for n in space)), "linear_attention")
+    forward_n, saved_n, work_n = (n.value for n in space)
+    parents = (q, k, v, log_decay) + ((state,) if state is not None else ())
+    train = _needs(*parents)
     out, final = DeviceArray(dev, (T, B, H, V)), DeviceArray(dev, (B, H, width, V))
-    saved = DeviceArray(dev, (saved_n.value,)) if saved_n.value else None
+    saved_n = saved_n if train else forward_n
+    saved = DeviceArray(dev, (saved_n,)) if saved_n else None
     d.out, d.final_state, d.saved = out.ptr, final.ptr, _p(saved)
     dev.call("ttrl_linear_attention_forward", C.byref(d))
-    parents = (q, k, v, log_decay) + ((state,) if state is not None else ())
-    if not _needs(*parents):
+    if not train:
         return _detached(out), _detached(final)
     outputs = Tensor(out, True, parents, "linear_attention")
     kept = (q.data, k.data, v.data, log_decay.data, state and state.data, done and done.data, saved, final)
@@ -119,7 +122,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: 
     def _backward(grad: DeviceArray):
         _q, _k, _v, _g, _s, _d, _saved, _final = kept  # alive until here
         grads = _Grads()
-        work = DeviceArray(dev, (max(1, work_n.value),))
+        work = DeviceArray(dev, (max(1, work_n),))
         arrays = [grads.array(t, t.shape, dev) for t in (q, k, v)]
         d.dout, d.dfinal, d.work = grad.ptr, _p(dfinal[0] if dfinal else None), work.ptr
         d.dq, d.dk, d.dv = (a.ptr for a in arrays)
