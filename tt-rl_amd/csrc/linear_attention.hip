@@ -157,6 +157,20 @@ __device__ __forceinline__ void step_decay(const SweepArgs& a, int t, int b, int
   }
 }
 
+// x of the lane N before, within 16 lanes; 0 where there is none.
+template <int N>
+__device__ __forceinline__ double before(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u)), 0x110 + N, 0xf, 0xf, true));
+  const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u >> 32)), 0x110 + N, 0xf, 0xf, true));
+  return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ double of_lane(double x, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane(uint32_t(u), lane), hi = __builtin_amdgcn_readlane(uint32_t(u >> 32), lane);
+  return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+
 // A chunk's decays, formed by one wavefront, row i of the sweep's order in lane i.
 struct Decays {
   double c[kChunk];    // sum of the log decays since the chunk's or the episode's start
@@ -169,27 +183,38 @@ struct Decays {
     const int i = lane & 31;
     const uint32_t starts = uint32_t(__ballot(reset));
     const uint32_t m = starts & (0xffffffffu >> (31 - i));
-    const int l = m ? 31 - __clz(m) : -1;
-    double s = reset ? 0.0 : double(g);
-#pragma unroll
-    for (int d = 1; d < kChunk; d <<= 1) {
-      const double t = __shfl_up(s, d, 32);
-      if (i - d >= max(l, 0)) s += t;
-    }
-    const double e = __shfl(s, 31, 32);
+    const int l = m ? 31 - __clz(m) : -1, from = max(l, 0);
+    double s = reset ? 0.0 : double(g), t;
+    // Sums over 1, 2, 4, 8 and 16 lanes that end here, down to the episode's start.
+    t = before<1>(s);
+    s = i - 1 >= from ? s + t : s;
+    t = before<2>(s);
+    s = i - 2 >= from ? s + t : s;
+    t = before<4>(s);
+    s = i - 4 >= from ? s + t : s;
+    t = before<8>(s);
+    s = i - 8 >= from ? s + t : s;
+    t = of_lane(s, 15);
+    s = i >= 16 && from < 16 ? s + t : s;
+    const double e = of_lane(s, 31);
     const int le = starts ? 31 - __clz(starts) : -1;
+    const float in = expf(float(s)), out = expf(float(e - s)), all = expf(float(e));
     if (lane < kChunk) {
       c[i] = s;
       lo[i] = l;
-      into[i] = expf(float(s));
-      left[i] = expf(float(e - s));
+      into[i] = in;
+      left[i] = out;
     }
     if (lane == 0) {
-      keep = le < 0 ? expf(float(e)) : 0.f;
+      keep = le < 0 ? all : 0.f;
       first = max(le, 0);
     }
   }
 };
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+template <class V>
+__device__ __forceinline__ V lds_at(const void* p) { return *reinterpret_cast<const V*>(p); }
 
 // 32 rows of an operand on their way into LDS, row r of the sweep's order.
 template <int KP, int NT, bool VEC>
@@ -224,9 +249,17 @@ struct Stage {
   }
 };
 
+// A scalar that stays in registers: without this the compiler reads kernel
+// arguments again where it needs them, a wait each time.
+template <class T>
+__device__ __forceinline__ void pin(T& x) {
+  asm volatile("" : "+s"(x));
+}
+
 // LOCAL: the first launch, what a segment adds to the state.
 template <int KP, int NW, bool VEC, bool LOCAL>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 128 && NW == 4 ? 2 : 3))) void k_sweep(SweepArgs a) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 128 ? 2 : 3))) void k_sweep(
+    SweepArgs a) {
   constexpr int NT = 64 * NW, KB = KP / 16, PX = KP + 4, PP = kChunk + 4;
   __shared__ __attribute__((aligned(16))) float lx[LOCAL ? 1 : 2][LOCAL ? 4 : kChunk * PX];
   __shared__ __attribute__((aligned(16))) float ly[2][kChunk * PX];
@@ -236,45 +269,63 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bh = int(blockIdx.x), b = bh / a.H, h = bh - b * a.H, run = int(blockIdx.y);
-  const int t0 = run * a.run, n = min(a.run, a.T - t0), back = w.back;
-  const int D = w.x.dim, E = w.z.dim, nkb = (D + 15) / 16, nch = (n + kChunk - 1) / kChunk;
+  const int t0 = run * a.run, n = min(a.run, a.T - t0);
+  int back = w.back, D = w.x.dim, E = w.z.dim, sk = w.sk, se = w.se;
+  float alpha_out = w.alpha_out, alpha_pair = w.alpha_pair;
+  float* marks = w.marks;
+  pin(back), pin(D), pin(E), pin(sk), pin(se), pin(alpha_out), pin(alpha_pair), pin(marks);
+  const int nch = (n + kChunk - 1) / kChunk;
   const int e = wave * 16 + lr;
   const bool cols = wave * 16 < E;  // uniform: this wavefront has columns of the state
   const long BH = long(a.B) * a.H;
 
   const Rows rx(w.x, a.B, b, h), ry(w.y, a.B, b, h), rz(w.z, a.B, b, h);
   const Rows ro(Operand{w.out, a.H, E, 1}, a.B, b, h);
+  const bool dotted = !LOCAL && w.dot.p;
+  const Rows rd(dotted ? w.dot : w.z, a.B, b, h);
   Stage<KP, NT, VEC> sx, sy;
   if constexpr (!LOCAL) sx.init(rx, back, tid);
   sy.init(ry, back, tid);
-  // Rows jb * 16 + 4 * lg + r of the sweep's order, this lane's column.
-  auto offset = [&](uint32_t pitch, int jb, int r) {
-    const int at = back ? (12 - 4 * lg) + (3 - r) + 16 * (1 - jb) : 4 * lg + r + 16 * jb;
-    return e < E ? uint32_t(at) * pitch + uint32_t(e) * 4u : kOut;
+  // Rows jb * 16 + 4 * lg + r of the sweep's order, this lane's column: a
+  // lane's part, formed where it is used (kept over the loop, these offsets
+  // would take more registers than the state), and a scalar part.
+  auto lane_part = [&](uint32_t pitch) {
+    int q = lg;
+    asm volatile("" : "+v"(q));
+    return e < E ? uint32_t(4 * (back ? 3 - q : q)) * pitch + uint32_t(e) * 4u : kOut;
   };
-  auto element = [&](int k, int r) {
-    const int d = k * 16 + 4 * lg + r;
-    return d < D && e < E ? uint32_t(d * w.sk + e * w.se) * 4u : kOut;
+  auto row_part = [&](uint32_t pitch, int jb, int r) {
+    return uint32_t(back ? (3 - r) + 16 * (1 - jb) : r + 16 * jb) * pitch;
   };
+  auto element = [&](int q, int k, int r) {
+    const int d = k * 16 + 4 * q + r;
+    return (d < D) & (e < E) ? uint32_t(d * sk + e * se) * 4u : kOut;
+  };
+  auto chunk_at = [&](int i) { return back ? nch - 1 - i : i; };  // i-th of the sweep
   float zn[2][4], gn = 0.f;
   bool fn = false;
-  auto fetch = [&](int c) {  // chunk c
-    const int t = t0 + c * kChunk, m = n - c * kChunk;
-    if constexpr (!LOCAL) sx.issue(rx.chunk(t, min(m, kChunk)));
-    sy.issue(ry.chunk(t, min(m, kChunk)));
-    const __amdgpu_buffer_rsrc_t r2 = rz.chunk(t, min(m, kChunk));
+  auto fetch_decays = [&](int i) {  // backwards a step's decay is the one of the step after it
+    const int s0 = chunk_at(i) * kChunk, j = lane & 31, s = s0 + (back ? kChunk - j : j), t = t0 + s;
+    const bool in = s < n + back && t < a.T;
+    const long at = in ? long(t) * a.B + b : 0;
+    const float g = a.g[a.g_rows ? at * a.H + h : long(h)], d = a.done ? a.done[at] : 0.f;
+    gn = in ? g : 0.f;
+    fn = in & ((d > 0.f) | (g < kForget));
+  };
+  auto fetch = [&](int i) {
+    const int s0 = chunk_at(i) * kChunk, t = t0 + s0, m = min(n - s0, kChunk);
+    if constexpr (!LOCAL) sx.issue(rx.chunk(t, m));
+    sy.issue(ry.chunk(t, m));
+    const __amdgpu_buffer_rsrc_t r2 = rz.chunk(t, m);
+    const uint32_t part = lane_part(rz.pitch);
 #pragma unroll
     for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) zn[jb][r] = load1(r2, offset(rz.pitch, jb, r));
-    if (wave == 0) {  // backwards a step's decay is the one of the step after it
-      const int i = lane & 31, s = back ? kChunk - i : i;
-      step_decay(a, t + s, b, h, gn, fn);
-      if (s >= m + back) gn = 0.f, fn = false;
-    }
+      for (int r = 0; r < 4; ++r) zn[jb][r] = load1(r2, part + row_part(rz.pitch, jb, r));
   };
   f32x4 S[KB];
-  fetch(back ? nch - 1 : 0);
+  if (wave == 0) fetch_decays(0);
+  fetch(0);
   {
     const bool any = !LOCAL && w.start && (w.start_all || (back ? t0 + n == a.T : t0 == 0));
     const __amdgpu_buffer_rsrc_t r0 =
@@ -282,27 +333,33 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) S[k][r] = load1(r0, element(k, r));
+      for (int r = 0; r < 4; ++r) S[k][r] = load1(r0, element(lg, k, r));
   }
   auto leave = [&](float* to, float scale, bool none) {
     const __amdgpu_buffer_rsrc_t r0 = resource(to, uint32_t(D) * E * 4u);
+    int q = lg;
+    asm volatile("" : "+v"(q));
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) store1(r0, element(k, r), none ? 0.f : S[k][r] * scale);
+      for (int r = 0; r < 4; ++r) store1(r0, element(q, k, r), none ? 0.f : S[k][r] * scale);
   };
+  if (wave == 0) {
+    ld[0].form(gn, fn, lane);
+    if (nch > 1) fetch_decays(1);
+  }
 
   float total = 1.f;
   for (int i = 0; i < nch; ++i) {
-    const int c = back ? nch - 1 - i : i, buf = i & 1;
+    const int c = chunk_at(i), buf = i & 1;
     float* X = lx[LOCAL ? 0 : buf];
     float* Y = ly[buf];
     float* P = lp[LOCAL ? 0 : buf];
-    Decays& dc = ld[buf];
+    const Decays& dc = ld[buf];
     if constexpr (!LOCAL) {
       sx.store(X, tid);
-      if (w.marks && (back ? i == 0 || (c + 1) * kChunk % a.seg == 0 : c * kChunk % a.seg == 0))
-        leave(w.marks + (c * kChunk / a.seg * BH + bh) * D * E, 1.f, false);
+      if (marks && (back ? i == 0 || (c + 1) * kChunk % a.seg == 0 : c * kChunk % a.seg == 0))
+        leave(marks + (c * kChunk / a.seg * BH + bh) * D * E, 1.f, false);
     }
     sy.store(Y, tid);
     float z[2][4];
@@ -310,30 +367,34 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
     for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) z[jb][r] = zn[jb][r];
-    if (wave == 0) dc.form(gn, fn, lane);
-    if (i + 1 < nch) fetch(back ? c - 1 : c + 1);
+    if (i + 1 < nch) fetch(i + 1);
     __syncthreads();
+    if (wave == 0 && i + 1 < nch) {
+      ld[buf ^ 1].form(gn, fn, lane);
+      if (i + 2 < nch) fetch_decays(i + 2);
+    }
 
     if constexpr (!LOCAL) {
       // Weights of the chunk's own rows: the three 16 x 16 blocks that have
       // any, by the last wavefronts (the ones without columns, if there are).
       for (int f = NW - 1 - wave; f < 3; f += NW) {
-        const int ri = f > 0, cj = f > 1, j = cj * 16 + lr;
-        f32x4 p = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int ri = f > 0, cj = f > 1, j = cj * 16 + lr, row = ri * 16 + 4 * lg;
+        const f64x2 c01 = lds_at<f64x2>(dc.c + row), c23 = lds_at<f64x2>(dc.c + row + 2);
+        const double cj0 = dc.c[j];
+        const i32x4 lo = lds_at<i32x4>(dc.lo + row);
+        f32x4 p[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int k = 0; k < KB; ++k) {
-          if (k >= nkb) break;
-          const f32x4 xa = *reinterpret_cast<const f32x4*>(X + (ri * 16 + lr) * PX + k * 16 + 4 * lg);
-          const f32x4 yb = *reinterpret_cast<const f32x4*>(Y + (cj * 16 + lr) * PX + k * 16 + 4 * lg);
+          const f32x4 xa = lds_at<f32x4>(X + (ri * 16 + lr) * PX + k * 16 + 4 * lg);
+          const f32x4 yb = lds_at<f32x4>(Y + (cj * 16 + lr) * PX + k * 16 + 4 * lg);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) p = mfma4(xa[r], yb[r], p);
+          for (int r = 0; r < 4; ++r) p[r & 1] = mfma4(xa[r], yb[r], p[r & 1]);
         }
-        const double cj0 = dc.c[j];
+        const double cr[4] = {c01.x, c01.y, c23.x, c23.y};
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = ri * 16 + 4 * lg + r;
-          const float wt = expf(float(dc.c[row] - cj0)) * (w.alpha_out * w.alpha_pair);
-          P[row * PP + j] = j <= row && j >= dc.lo[row] ? p[r] * wt : 0.f;
+          const float wt = expf(float(cr[r] - cj0)) * (alpha_out * alpha_pair);
+          P[(row + r) * PP + j] = (j <= row + r) & (j >= lo[r]) ? (p[0][r] + p[1][r]) * wt : 0.f;
         }
       }
       // What the entering state gives each row.
@@ -343,81 +404,87 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
       if (cols) {
 #pragma unroll
         for (int k = 0; k < KB; ++k) {
-          if (k >= nkb) break;
           f32x4 xa[2];
 #pragma unroll
-          for (int f = 0; f < 2; ++f) xa[f] = *reinterpret_cast<const f32x4*>(X + (f * 16 + lr) * PX + k * 16 + 4 * lg);
+          for (int f = 0; f < 2; ++f) xa[f] = lds_at<f32x4>(X + (f * 16 + lr) * PX + k * 16 + 4 * lg);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int f = 0; f < 2; ++f) o[f] = mfma4(xa[f][r], S[k][r], o[f]);
         }
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
+        for (int f = 0; f < 2; ++f) {
+          const i32x4 lo = lds_at<i32x4>(dc.lo + f * 16 + 4 * lg);
+          const f32x4 in = lds_at<f32x4>(dc.into + f * 16 + 4 * lg);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int row = f * 16 + 4 * lg + r;
-            o[f][r] = dc.lo[row] < 0 ? o[f][r] * (dc.into[row] * w.alpha_out) : 0.f;
+            const float x = o[f][r] * (in[r] * alpha_out);
+            o[f][r] = lo[r] < 0 ? x : 0.f;
           }
+        }
       }
       __syncthreads();
       if (cols) {
+        const int t = t0 + c * kChunk, m = min(n - c * kChunk, kChunk);
+        float d[2][4];
+        if (dotted) {
+          const __amdgpu_buffer_rsrc_t r3 = rd.chunk(t, m);
+          const uint32_t part = lane_part(rd.pitch);
+#pragma unroll
+          for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d[f][r] = load1(r3, part + row_part(rd.pitch, f, r));
+        }
         bool odd = false;
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) odd = odd || !finite(z[jb][r]);
+          for (int r = 0; r < 4; ++r) odd |= !finite(z[jb][r]);
         if (!__any(odd)) {
+          f32x4 pa[3];
 #pragma unroll
-          for (int jb = 0; jb < 2; ++jb) {
-            f32x4 pa[2];
+          for (int f = 0; f < 3; ++f) pa[f] = lds_at<f32x4>(P + ((f > 0) * 16 + lr) * PP + (f > 1) * 16 + 4 * lg);
 #pragma unroll
-            for (int f = jb; f < 2; ++f) pa[f] = *reinterpret_cast<const f32x4*>(P + (f * 16 + lr) * PP + jb * 16 + 4 * lg);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-              for (int f = jb; f < 2; ++f) o[f] = mfma4(pa[f][r], z[jb][r], o[f]);
+          for (int r = 0; r < 4; ++r) {
+            o[0] = mfma4(pa[0][r], z[0][r], o[0]);
+            o[1] = mfma4(pa[1][r], z[0][r], o[1]);
           }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[1] = mfma4(pa[2][r], z[1][r], o[1]);
         } else {
-#pragma unroll
-          for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
+          // z again, row by row, for the rows that see it
+          const __amdgpu_buffer_rsrc_t r2 = rz.chunk(t, m);
 #pragma unroll 1
-              for (int m = 0; m < 4; ++m) {
-                const int j = jb * 16 + 4 * m + r;
-                const float zj = __shfl(z[jb][r], lr + 16 * m, 64);
+          for (int j = 0; j < kChunk; ++j) {
+            const float zj = load1(r2, e < E ? uint32_t(back ? kChunk - 1 - j : j) * rz.pitch + uint32_t(e) * 4u : kOut);
 #pragma unroll
-                for (int f = jb; f < 2; ++f)
+            for (int f = 0; f < 2; ++f) {
+              const i32x4 lo = lds_at<i32x4>(dc.lo + f * 16 + 4 * lg);
 #pragma unroll
-                  for (int q = 0; q < 4; ++q) {
-                    const int row = f * 16 + 4 * lg + q;
-                    if (j <= row && j >= dc.lo[row]) o[f][q] += P[row * PP + j] * zj;
-                  }
+              for (int r = 0; r < 4; ++r) {
+                const int row = f * 16 + 4 * lg + r;
+                const bool sees = (j <= row) & (j >= lo[r]);
+                const float x = o[f][r] + (sees ? P[row * PP + j] : 0.f) * zj;
+                o[f][r] = sees ? x : o[f][r];
               }
+            }
+          }
         }
-        const int t = t0 + c * kChunk, m = min(n - c * kChunk, kChunk);
         const __amdgpu_buffer_rsrc_t r2 = ro.chunk(t, m);
+        const uint32_t part = lane_part(ro.pitch);
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) store1(r2, offset(ro.pitch, f, r), o[f][r]);
-        if (w.dot.p) {
-          const Rows rd(w.dot, a.B, b, h);
-          const __amdgpu_buffer_rsrc_t r3 = rd.chunk(t, m);
-          float* to = w.dots + (long(wave) * BH + bh) * a.T + t;
-          float d[2][4];
-#pragma unroll
-          for (int f = 0; f < 2; ++f)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) d[f][r] = load1(r3, offset(rd.pitch, f, r)) * o[f][r];
+          for (int r = 0; r < 4; ++r) store1(r2, part + row_part(ro.pitch, f, r), o[f][r]);
+        if (dotted) {
+          const __amdgpu_buffer_rsrc_t r4 = resource(w.dots + (long(wave) * BH + bh) * a.T + t, uint32_t(m) * 4u);
 #pragma unroll
           for (int f = 0; f < 2; ++f)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const int row = f * 16 + 4 * lg + r, s = back ? kChunk - 1 - row : row;
-              const float sum = row_sum(e < E ? d[f][r] : 0.f);
-              if (lr == 0 && s < m) to[s] = sum;
+              const float sum = row_sum(e < E ? d[f][r] * o[f][r] : 0.f);
+              store1(r4, lr == 0 ? uint32_t(s) * 4u : kOut, sum);
             }
         }
       }
@@ -426,42 +493,42 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
     // The state on leaving the chunk.
     const float keep = dc.keep;
     const int first = __builtin_amdgcn_readfirstlane(dc.first);
-    total *= keep;
+    if constexpr (LOCAL) total *= keep;
     if (cols) {
 #pragma unroll
-      for (int k = 0; k < KB; ++k)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[k][r] = keep == 0.f ? 0.f : S[k][r] * keep;
-#pragma unroll
-      for (int jb = 0; jb < 2; ++jb)
+      for (int jb = 0; jb < 2; ++jb) {
+        const f32x4 left = lds_at<f32x4>(dc.left + jb * 16 + 4 * lg);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = jb * 16 + 4 * lg + r;
-          z[jb][r] = j >= first ? z[jb][r] * (dc.left[j] * w.alpha_pair) : 0.f;
+          const float x = z[jb][r] * (left[r] * alpha_pair);
+          z[jb][r] = j >= first ? x : 0.f;
         }
-      if (first == 0) {
+      }
 #pragma unroll
-        for (int k = 0; k < KB; ++k) {
-          if (k >= nkb) break;
+      for (int k = 0; k < KB; ++k)
 #pragma unroll
-          for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              S[k] = mfma4(Y[(jb * 16 + 4 * lg + r) * PX + k * 16 + lr], z[jb][r], S[k]);
+        for (int r = 0; r < 4; ++r) {
+          const float x = S[k][r] * keep;
+          S[k][r] = keep == 0.f ? 0.f : x;
         }
-      } else {  // rows before `first` are another episode's
 #pragma unroll
-        for (int k = 0; k < KB; ++k) {
-          if (k >= nkb) break;
+      for (int jb = 0; jb < 2; ++jb) {
+        float y[KB][4];
 #pragma unroll
-          for (int jb = 0; jb < 2; ++jb)
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int j = jb * 16 + 4 * lg + r;
-              const float y = Y[j * PX + k * 16 + lr];
-              S[k] = mfma4(j >= first ? y : 0.f, z[jb][r], S[k]);
-            }
+          for (int k = 0; k < KB; ++k) y[k][r] = Y[(jb * 16 + 4 * lg + r) * PX + k * 16 + lr];
+        if (first > 0) {  // rows before `first` are another episode's
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int k = 0; k < KB; ++k) y[k][r] = jb * 16 + 4 * lg + r >= first ? y[k][r] : 0.f;
         }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int k = 0; k < KB; ++k) S[k] = mfma4(y[k][r], z[jb][r], S[k]);
       }
     }
   }
