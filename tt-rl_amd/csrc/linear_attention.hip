@@ -48,7 +48,9 @@
 // values forms its inner sums over the allowed steps alone.
 #include "common.hpp"
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace ttrl {
 namespace {
@@ -141,8 +143,8 @@ struct Rows {
     pitch = uint32_t(B) * uint32_t(o.heads) * uint32_t(o.dim) * 4u;
     width = uint32_t(o.dim) * 4u;
   }
-  __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk(int t, int n) const {  // n > 0 steps from t on
-    return resource(reinterpret_cast<const char*>(p) + long(t) * pitch, uint32_t(n - 1) * pitch + width);
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk(int t, int n) const {  // n steps from t on
+    return resource(reinterpret_cast<const char*>(p) + long(t) * pitch, n > 0 ? uint32_t(n - 1) * pitch + width : 0u);
   }
 };
 
@@ -171,9 +173,12 @@ __device__ __forceinline__ double of_lane(double x, int lane) {
   return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
 }
 
+// 2^x, zero below float32's normal range.
+__device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // A chunk's decays, formed by one wavefront, row i of the sweep's order in lane i.
 struct Decays {
-  double c[kChunk];    // sum of the log decays since the chunk's or the episode's start
+  double c[kChunk];    // sum of the decays' logarithms (to base 2) since the chunk's or the episode's start
   float into[kChunk];  // weight of the state on entering the chunk (where lo < 0)
   float left[kChunk];  // weight of the row in the state on leaving it (from `first` on)
   int lo[kChunk];      // the episode's first row in the chunk, -1: before it
@@ -184,7 +189,7 @@ struct Decays {
     const uint32_t starts = uint32_t(__ballot(reset));
     const uint32_t m = starts & (0xffffffffu >> (31 - i));
     const int l = m ? 31 - __clz(m) : -1, from = max(l, 0);
-    double s = reset ? 0.0 : double(g), t;
+    double s = reset ? 0.0 : double(g) * 1.4426950408889634074, t;
     // Sums over 1, 2, 4, 8 and 16 lanes that end here, down to the episode's start.
     t = before<1>(s);
     s = i - 1 >= from ? s + t : s;
@@ -198,7 +203,7 @@ struct Decays {
     s = i >= 16 && from < 16 ? s + t : s;
     const double e = of_lane(s, 31);
     const int le = starts ? 31 - __clz(starts) : -1;
-    const float in = expf(float(s)), out = expf(float(e - s)), all = expf(float(e));
+    const float in = power(float(s)), out = power(float(e - s)), all = power(float(e));
     if (lane < kChunk) {
       c[i] = s;
       lo[i] = l;
@@ -273,7 +278,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
   int back = w.back, D = w.x.dim, E = w.z.dim, sk = w.sk, se = w.se;
   float alpha_out = w.alpha_out, alpha_pair = w.alpha_pair;
   float* marks = w.marks;
-  pin(back), pin(D), pin(E), pin(sk), pin(se), pin(alpha_out), pin(alpha_pair), pin(marks);
+  const float* done = a.done;
+  int g_rows = a.g_rows;
+  pin(done), pin(g_rows), pin(back), pin(D), pin(E), pin(sk), pin(se), pin(alpha_out), pin(alpha_pair), pin(marks);
   const int nch = (n + kChunk - 1) / kChunk;
   const int e = wave * 16 + lr;
   const bool cols = wave * 16 < E;  // uniform: this wavefront has columns of the state
@@ -286,45 +293,62 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
   Stage<KP, NT, VEC> sx, sy;
   if constexpr (!LOCAL) sx.init(rx, back, tid);
   sy.init(ry, back, tid);
-  // Rows jb * 16 + 4 * lg + r of the sweep's order, this lane's column: a
-  // lane's part, formed where it is used (kept over the loop, these offsets
-  // would take more registers than the state), and a scalar part.
-  auto lane_part = [&](uint32_t pitch) {
+  // Rows jb * 16 + 4 * lg + r of the sweep's order, this lane's column; formed
+  // where they are used (kept over the loop they would take more registers
+  // than the state), from the first by steps of one row.
+  struct Offsets {
+    uint32_t at[2][4];
+  };
+  auto offsets = [&](uint32_t pitch) __attribute__((always_inline)) {
     int q = lg;
     asm volatile("" : "+v"(q));
-    return e < E ? uint32_t(4 * (back ? 3 - q : q)) * pitch + uint32_t(e) * 4u : kOut;
-  };
-  auto row_part = [&](uint32_t pitch, int jb, int r) {
-    return uint32_t(back ? (3 - r) + 16 * (1 - jb) : r + 16 * jb) * pitch;
-  };
-  auto element = [&](int q, int k, int r) {
-    const int d = k * 16 + 4 * q + r;
-    return (d < D) & (e < E) ? uint32_t(d * sk + e * se) * 4u : kOut;
-  };
-  auto chunk_at = [&](int i) { return back ? nch - 1 - i : i; };  // i-th of the sweep
-  float zn[2][4], gn = 0.f;
-  bool fn = false;
-  auto fetch_decays = [&](int i) {  // backwards a step's decay is the one of the step after it
-    const int s0 = chunk_at(i) * kChunk, j = lane & 31, s = s0 + (back ? kChunk - j : j), t = t0 + s;
-    const bool in = s < n + back && t < a.T;
-    const long at = in ? long(t) * a.B + b : 0;
-    const float g = a.g[a.g_rows ? at * a.H + h : long(h)], d = a.done ? a.done[at] : 0.f;
-    gn = in ? g : 0.f;
-    fn = in & ((d > 0.f) | (g < kForget));
-  };
-  auto fetch = [&](int i) {
-    const int s0 = chunk_at(i) * kChunk, t = t0 + s0, m = min(n - s0, kChunk);
-    if constexpr (!LOCAL) sx.issue(rx.chunk(t, m));
-    sy.issue(ry.chunk(t, m));
-    const __amdgpu_buffer_rsrc_t r2 = rz.chunk(t, m);
-    const uint32_t part = lane_part(rz.pitch);
+    const uint32_t by = back ? 0u - pitch : pitch, top = back ? uint32_t(kChunk - 1) * pitch : 0u;
+    Offsets f;
+    f.at[0][0] = top + (e < E ? uint32_t(4 * q) * by + uint32_t(e) * 4u : kOut);
+    f.at[1][0] = f.at[0][0] + 16u * by;
 #pragma unroll
     for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) zn[jb][r] = load1(r2, part + row_part(rz.pitch, jb, r));
+      for (int r = 1; r < 4; ++r) f.at[jb][r] = f.at[jb][r - 1] + by;
+    return f;
+  };
+  auto element = [&](int q, int k, int r) __attribute__((always_inline)) {
+    const int d = k * 16 + 4 * q + r;
+    return (d < D) & (e < E) ? uint32_t(d * sk + e * se) * 4u : kOut;
+  };
+  auto chunk_at = [&](int i) __attribute__((always_inline)) { return back ? nch - 1 - i : i; };  // i-th of the sweep
+  // A chunk's loads on their way; every wavefront takes the same ones, the
+  // decays' a chunk earlier than the rows', so that none is waited for early.
+  float zn[2][4], gn, dn;
+  const uint32_t gp = g_rows ? uint32_t(a.B) * uint32_t(a.H) * 4u : 0u, dp = uint32_t(a.B) * 4u;
+  const int shift = lane & 31, step = back ? kChunk - shift : shift;  // backwards a step's decay is that of the step after it
+  auto fetch_decays = [&](int i) __attribute__((always_inline)) {
+    const int t = t0 + (i < nch ? chunk_at(i) * kChunk : 0), left = i < nch ? min(a.T - t, kChunk + 1) : 0;
+    const float* g = a.g + (g_rows ? (long(t) * a.B + b) * a.H + h : long(h));
+    gn = load1(resource(g, left > 0 ? uint32_t(left - 1) * gp + 4u : 0u), uint32_t(step) * gp);
+    dn = load1(resource(done ? done + long(t) * a.B + b : g, done && left > 0 ? uint32_t(left - 1) * dp + 4u : 0u),
+               uint32_t(step) * dp);
+  };
+  auto form = [&](Decays& d, int i, float g, float ended) __attribute__((always_inline)) {
+    const int s = chunk_at(i) * kChunk + step;
+    const bool in = (i < nch) & (s < n + back) & (t0 + s < a.T);
+    d.form(in ? g : 0.f, in & ((ended > 0.f) | (g < kForget)), lane);
+  };
+  auto fetch = [&](int i) __attribute__((always_inline)) {
+    const int s0 = i < nch ? chunk_at(i) * kChunk : 0, t = t0 + s0, m = i < nch ? min(n - s0, kChunk) : 0;
+    if constexpr (!LOCAL) sx.issue(rx.chunk(t, m));
+    sy.issue(ry.chunk(t, m));
+    const __amdgpu_buffer_rsrc_t r2 = rz.chunk(t, m);
+    const Offsets f = offsets(rz.pitch);
+#pragma unroll
+    for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) zn[jb][r] = load1(r2, f.at[jb][r]);
+    fetch_decays(i + 1);
   };
   f32x4 S[KB];
-  if (wave == 0) fetch_decays(0);
+  fetch_decays(0);
+  float gc = gn, ec = dn;
   fetch(0);
   {
     const bool any = !LOCAL && w.start && (w.start_all || (back ? t0 + n == a.T : t0 == 0));
@@ -335,7 +359,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
 #pragma unroll
       for (int r = 0; r < 4; ++r) S[k][r] = load1(r0, element(lg, k, r));
   }
-  auto leave = [&](float* to, float scale, bool none) {
+  auto leave = [&](float* to, float scale, bool none) __attribute__((always_inline)) {
     const __amdgpu_buffer_rsrc_t r0 = resource(to, uint32_t(D) * E * 4u);
     int q = lg;
     asm volatile("" : "+v"(q));
@@ -344,10 +368,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
 #pragma unroll
       for (int r = 0; r < 4; ++r) store1(r0, element(q, k, r), none ? 0.f : S[k][r] * scale);
   };
-  if (wave == 0) {
-    ld[0].form(gn, fn, lane);
-    if (nch > 1) fetch_decays(1);
-  }
+  if (wave == 0) form(ld[0], 0, gc, ec);
 
   float total = 1.f;
   for (int i = 0; i < nch; ++i) {
@@ -366,12 +387,26 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
 #pragma unroll
     for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) z[jb][r] = zn[jb][r];
-    if (i + 1 < nch) fetch(i + 1);
+      for (int r = 0; r < 4; ++r) {
+        z[jb][r] = zn[jb][r];
+        asm volatile("" : "+v"(z[jb][r]));
+      }
+    gc = gn;
+    ec = dn;
+    asm volatile("" : "+v"(gc), "+v"(ec));  // moved before the loads below
+    fetch(i + 1);
     __syncthreads();
-    if (wave == 0 && i + 1 < nch) {
-      ld[buf ^ 1].form(gn, fn, lane);
-      if (i + 2 < nch) fetch_decays(i + 2);
+    if (wave == 0) form(ld[buf ^ 1], i + 1, gc, ec);
+
+    const int t = t0 + c * kChunk, m = min(n - c * kChunk, kChunk);
+    float d[2][4];
+    if (dotted) {
+      const __amdgpu_buffer_rsrc_t r3 = rd.chunk(t, m);
+      const Offsets at = offsets(rd.pitch);
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) d[f][r] = load1(r3, at.at[f][r]);
     }
 
     if constexpr (!LOCAL) {
@@ -393,8 +428,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
         const double cr[4] = {c01.x, c01.y, c23.x, c23.y};
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float wt = expf(float(cr[r] - cj0)) * (alpha_out * alpha_pair);
-          P[(row + r) * PP + j] = (j <= row + r) & (j >= lo[r]) ? (p[0][r] + p[1][r]) * wt : 0.f;
+          float x = (p[0][r] + p[1][r]) * (power(float(cr[r] - cj0)) * (alpha_out * alpha_pair));
+          asm volatile("" : "+v"(x));  // a select, not a branch round the exponential
+          P[(row + r) * PP + j] = (j <= row + r) & (j >= lo[r]) ? x : 0.f;
         }
       }
       // What the entering state gives each row.
@@ -425,16 +461,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
       }
       __syncthreads();
       if (cols) {
-        const int t = t0 + c * kChunk, m = min(n - c * kChunk, kChunk);
-        float d[2][4];
-        if (dotted) {
-          const __amdgpu_buffer_rsrc_t r3 = rd.chunk(t, m);
-          const uint32_t part = lane_part(rd.pitch);
-#pragma unroll
-          for (int f = 0; f < 2; ++f)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) d[f][r] = load1(r3, part + row_part(rd.pitch, f, r));
-        }
         bool odd = false;
 #pragma unroll
         for (int jb = 0; jb < 2; ++jb)
@@ -470,12 +496,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
             }
           }
         }
-        const __amdgpu_buffer_rsrc_t r2 = ro.chunk(t, m);
-        const uint32_t part = lane_part(ro.pitch);
-#pragma unroll
-        for (int f = 0; f < 2; ++f)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) store1(r2, part + row_part(ro.pitch, f, r), o[f][r]);
         if (dotted) {
           const __amdgpu_buffer_rsrc_t r4 = resource(w.dots + (long(wave) * BH + bh) * a.T + t, uint32_t(m) * 4u);
 #pragma unroll
@@ -487,6 +507,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 1
               store1(r4, lr == 0 ? uint32_t(s) * 4u : kOut, sum);
             }
         }
+        const __amdgpu_buffer_rsrc_t r2 = ro.chunk(t, m);
+        const Offsets at = offsets(ro.pitch);
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) store1(r2, at.at[f][r], o[f][r]);
       }
     }
 
