@@ -883,7 +883,8 @@ int ttrl_linear_attention_token(ttrl_ctx* ctx, int B, int H, int kv_heads, int K
 /* The gated projections of a feed-forward block (no counterpart in the
  * reference): h = act(x W_gate + b_gate) * (x W_up + b_up), x [M][K], weights
  * [K][N] (in, out), biases [N] or NULL, h [M][N].  g and u, both or neither,
- * receive the two projections for the backward.  act: */
+ * receive the two projections for the backward.  Operands hold fewer than
+ * 2^29 values.  act: */
 #define TTRL_GATE_SILU 0
 #define TTRL_GATE_GELU 1 /* with the error function */
 #define TTRL_GATE_RELU 2
@@ -898,11 +899,22 @@ typedef struct ttrl_gated_desc {
   float* g;
   float* u;
   float* h;
+  void* work;
+  const float* dh;
+  float* dx;
+  float* dw_gate;
+  float* dw_up;
+  float* db_gate;
+  float* db_up;
 } ttrl_gated_desc;
+/* Bytes of `work`, on 16 bytes, that the forward and the backward use (the
+ * forward's may be NULL where 0). */
+int ttrl_gated_space(const ttrl_gated_desc* desc, long* forward_bytes, long* backward_bytes);
 int ttrl_gated_forward(ttrl_ctx* ctx, const ttrl_gated_desc* desc);
-/* dg = dh * u * act'(g), du = dh * act(g), all [M][N]. */
-int ttrl_gated_slopes(ttrl_ctx* ctx, int M, int N, int act, const float* dh, const float* g, const float* u, float* dg,
-                      float* du);
+/* dx = (dh * u * act'(g)) W_gate^T + (dh * act(g)) W_up^T and the gradients of
+ * the weights and biases, from the forward's g and u; each is overwritten, or
+ * not formed where NULL. */
+int ttrl_gated_backward(ttrl_ctx* ctx, const ttrl_gated_desc* desc);
 
 /* AdamW over many tensors in one launch per 64 (the reference's Adam,
  * ttrl/engine/optim/adam.py:25-134, has coupled decay and 32-bit states):

@@ -157,7 +157,8 @@ class GatedDesc(C.Structure):
     """Mirror of ttrl_gated_desc."""
 
     _fields_ = ([(n, C.c_int) for n in ("M", "K", "N", "act")]
-                + [(n, C.c_void_p) for n in ("x", "w_gate", "w_up", "b_gate", "b_up", "g", "u", "h")])
+                + [(n, C.c_void_p) for n in ("x", "w_gate", "w_up", "b_gate", "b_up", "g", "u", "h", "work", "dh", "dx",
+                                             "dw_gate", "dw_up", "db_gate", "db_up")])
 
 
 ADAMW_COUNTER_BYTES = 24
@@ -316,7 +317,8 @@ SIGNATURES = {
     "ttrl_linear_attention_backward": ([P, C.POINTER(LinearAttentionDesc)], I),
     "ttrl_linear_attention_token": ([P, I, I, I, I, I, P, P, P, P, I, P, F, P, P], I),
     "ttrl_gated_forward": ([P, C.POINTER(GatedDesc)], I),
-    "ttrl_gated_slopes": ([P, I, I, I, P, P, P, P, P], I),
+    "ttrl_gated_space": ([C.POINTER(GatedDesc), C.POINTER(L), C.POINTER(L)], I),
+    "ttrl_gated_backward": ([P, C.POINTER(GatedDesc)], I),
     "ttrl_adamw_set_count": ([P, P, I, C.c_double, C.c_double], I),
     "ttrl_adamw_step": ([P, I, C.POINTER(AdamWTensor), I, P, P, P, P, P, C.c_double, C.c_double, C.c_double, C.c_double,
                          C.c_double], I),

@@ -188,47 +188,27 @@ def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Tensor | None 
         if t is not None and t.dtype != np.float32:
             raise ValueError(f"{who}: {name} must be float32, got {t.dtype}")
     dev, train = x.device, _needs(*tensors)
-    act = _lib.GATES[activation]
     h = DeviceArray(dev, (M, N))
     g, u = (DeviceArray(dev, (M, N)) for _ in range(2)) if train else (None, None)
-    dev.call("ttrl_gated_forward", C.byref(_lib.GatedDesc(M, width, N, act, *(_p(t) for t in tensors), _p(g), _p(u), h.ptr)))
+    d = _lib.GatedDesc(M, width, N, _lib.GATES[activation], *(_p(t) for t in tensors), _p(g), _p(u), h.ptr)
+    forward_n, backward_n = C.c_long(), C.c_long()
+    _lib.check(_lib.lib().ttrl_gated_space(C.byref(d), C.byref(forward_n), C.byref(backward_n)), who)
+    work = DeviceArray(dev, (forward_n.value,), np.uint8) if forward_n.value else None
+    d.work = _p(work)
+    dev.call("ttrl_gated_forward", C.byref(d))
     if not train:
         return _detached(h)
     out = Tensor(h, True, tuple(t for t in tensors if t is not None), "gated_linear")
-    x_data, weights = x.data, (w_gate.data, w_up.data)
+    kept = (x.data, w_gate.data, w_up.data, g, u)
 
     def _backward(grad: DeviceArray):
-        dgu = [DeviceArray(dev, (M, N)) for _ in range(2)]
-        dev.call("ttrl_gated_slopes", M, N, act, grad.vp, g.vp, u.vp, dgu[0].vp, dgu[1].vp)
-        dx, beta_x = x._grad_target() if x.requires_grad else (None, 0.0)
-        if dx is not None:
-            x._note_write(beta_x, False)
-        for w, data, bias, dy in ((w_gate, weights[0], b_gate, dgu[0]), (w_up, weights[1], b_up, dgu[1])):
-            _linear_grads(dev, M, width, N, x_data, data, dy, w, bias, dx, beta_x)
-            beta_x = 1.0
+        _kept, grads = kept, _Grads()  # alive until here
+        work = DeviceArray(dev, (max(1, backward_n.value),), np.uint8)
+        d.work, d.dh = work.ptr, grad.ptr
+        d.dx, d.dw_gate, d.dw_up, d.db_gate, d.db_up = (
+            grads.array(t).ptr if t is not None and t.requires_grad else None for t in tensors)
+        dev.call("ttrl_gated_backward", C.byref(d))
+        grads.settle()
 
     out._backward = _backward
     return out
-
-
-def _linear_grads(dev, M, width, N, x, w_data, dy, w, bias, dx, beta_x) -> None:
-    from ttrl_amd.engine.ops.fused import grad_targets
-
-    (dw, db), beta_w = grad_targets(w, bias)
-    if dw is None and db is not None:  # the bias alone: a column sum
-        s = K.reduce_dim("sum", dy, 0, keepdim=True).reshape(db.shape)
-        K.binary_into("add", db, s, db) if beta_w else db.copy_from(s)
-        db = None
-    if M == 0:
-        for a in (dw, db):
-            if a is not None and not beta_w:
-                a.fill(0.0)
-        return
-    if dw is None and dx is None:
-        return
-    b = _lib.LinearDesc()
-    b.M, b.K, b.N, b.groups = M, width, N, 1
-    b.x, b.ldx, b.W, b.dy = x.ptr, width, w_data.ptr, dy.ptr
-    b.dW, b.db, b.dx, b.lddx = _p(dw), _p(db), _p(dx), width
-    b.beta_w, b.beta_x = beta_w, beta_x
-    dev.call("ttrl_linear_backward", C.byref(b))
