@@ -13,17 +13,32 @@
 // Few rows (an acting step) only read the weights once: k_few takes them
 // straight from memory into FP32 MFMA.
 //
-// Otherwise the products run on the bf16 matrix cores as FP32 products: a
-// float is exactly the sum of three bf16, and of the nine products of two
-// floats' parts the six largest are kept (split_gemm.hpp has the bounds and
-// the reference).  Unlike the convolutions' core there, which splits operands as it
-// stages them, operands are split once, by k_pack, into the very order in
-// which the matrix cores take them: 16 rows x 32 k of one part are 1 KiB,
+// Otherwise the products run on the fp16 matrix cores.  Every row of an operand
+// (the values that one output sums over) is scaled by a power of two, so that
+// its largest value lies in [2^14, 2^15), and each value v is split into
+//
+//   h = v to the nearest fp16,  l = v - h to the nearest fp16,
+//
+// 11 significant bits each, of either sign: v - h - l is at most 2^-23 of v's
+// power of two.  Of the four products of two values' parts hh, hl and lh are
+// kept; ll is at most 2^-22 of the product, of either sign.  Together a product
+// is off by 2^-21 at worst and 2^-24 in the mean, as one rounding of FP32 is,
+// every partial product is exact in FP32 and added in FP32, hh apart from the
+// other two, so the main sum is rounded once per 32 k.  fp16 ends at 2^-24, so a
+// value under 2^-2 (2^-16 of its row's largest) is off by up to 2^-25 instead;
+// such values are counted by row, and where that count could show in a sum
+// (lossy() below), or a sum is not finite, it is formed again in FP32.
+//
+// (Three bf16 parts, 24 bits at any exponent, need six products and no scale:
+// 8192 x 1024 x 4096 forward and backward took 2651 us instead of @8192@.)
+//
+// Operands are split once, by k_pack, into the very order in which the matrix
+// cores take them: 16 rows x 32 k of one part are 1 KiB,
 //   [block of 16 rows][step of 32 k][part][k / 8][row][8 k],
 // so k_mma moves whole fragments from memory to LDS without a register and
-// reads them without conflicts, and every part is split once however many
-// tiles read it.  Packing writes 6 bytes a value beside the 4 read; a product
-// reads each value M / 128 or N / 128 times.
+// reads them without conflicts, and every value is split once however many
+// tiles read it.  The scales cost one more pass over what is packed (k_scan);
+// packing writes 4 bytes a value beside the 4 read.
 #include "split_gemm.hpp"
 
 #include <algorithm>
@@ -99,7 +114,7 @@ __device__ float element_b(const Source& s, int product, int n, int k) {
   return k < s.M ? s.slope_of(k, c, up) : 0.f;
 }
 
-constexpr int kPart = 1024, kFrag = 3 * kPart;  // bytes of 16 x 32 values: a part, all three
+constexpr int kParts = 2, kPart = 1024, kFrag = kParts * kPart;  // bytes of 16 x 32 values: a part, both
 
 // A matrix packed by rows (k along its columns) and by columns (k along its
 // rows), either or both.  Block b of 16 rows, step s of 32 k is fragment
@@ -107,29 +122,160 @@ constexpr int kPart = 1024, kFrag = 3 * kPart;  // bytes of 16 x 32 values: a pa
 struct Packed {
   char* p;
   int steps, first, mul, add;
+  int2* rows;  // of packed row r: the exponent of its largest value less 14; how many values fp16 ends above
 };
 struct PackJob {
   const float* src;  // plain matrix (R, C), or null: both slopes of the Source
   int R, C;
-  Packed rows[2], cols[2];  // of the gate and of the up slopes; a plain matrix has the first
-  float* sums;              // [R / 32][2][C] column sums of the slopes, or null
-  int tiles_c, block0;
+  Packed rows[2], cols[2];        // of the gate and of the up slopes; a plain matrix has the first
+  uint32_t *row_max, *col_max;    // largest magnitudes (bits) of the scan's tiles: [tile column][R], [part][tile row][C]
+  float* sums;                    // [R / 32][2][C] column sums of the slopes, or null
+  int tiles_c, block0, scan_c, scan0;
 };
-constexpr int kJobs = 3, kPackR = 32, kPackC = 64;
+constexpr int kJobs = 4, kPackR = 32, kPackC = 64, kScanR = 64, kScanC = 128;
 struct PackArgs {
   PackJob job[kJobs];
   int jobs;
   Source s;
 };
 
-// A lane's 8 values of a fragment, split.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// The largest magnitudes of 64 x 128 values by row and by column.  NaN and
+// infinity count as the largest.  A wavefront has 16 rows, 8 (of slopes 4) of
+// them in flight.
+template <bool SLOPES>
+__device__ __forceinline__ void scan_tile(const PackJob& j, const Source& s, int tr, int tc, uint32_t (*top)[4][kScanC]) {
+  constexpr int NC = kScanC / 64, PARTS = SLOPES ? 2 : 1, DEEP = SLOPES ? 4 : 8;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int R = j.R, C = j.C, c0 = tc * kScanC, r0 = tr * kScanR + wave * (kScanR / 4);
+  uint32_t col[PARTS][NC] = {};
+#pragma unroll 1
+  for (int d = 0; d < kScanR / 4; d += DEEP) {
+    float v[SLOPES ? 3 : 1][DEEP][NC];
+    uint32_t row[DEEP] = {}, m[DEEP][NC][PARTS];
+#pragma unroll
+    for (int y = 0; y < DEEP; ++y)
+#pragma unroll
+      for (int x = 0; x < NC; ++x) {  // the last row and column again where the matrix ends
+        const long at = long(min(r0 + d + y, R - 1)) * C + min(c0 + x * 64 + lane, C - 1);
+        if constexpr (SLOPES) {
+          v[0][y][x] = s.g[at];
+          v[1][y][x] = s.u[at];
+          v[2][y][x] = s.dh[at];
+        } else {
+          v[0][y][x] = j.src[at];
+        }
+      }
+#pragma unroll
+    for (int y = 0; y < DEEP; ++y)
+#pragma unroll
+      for (int x = 0; x < NC; ++x) {
+        if constexpr (SLOPES) {
+          float slope;
+          const float act = gate(s.act, v[0][y][x], &slope);
+          m[y][x][0] = magnitude(v[2][y][x] * v[1][y][x] * slope);
+          m[y][x][1] = magnitude(v[2][y][x] * act);
+        } else {
+          m[y][x][0] = magnitude(v[0][y][x]);
+        }
+      }
+#pragma unroll
+    for (int y = 0; y < DEEP; ++y)
+#pragma unroll
+      for (int x = 0; x < NC; ++x)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          row[y] = max(row[y], m[y][x][p]);
+          col[p][x] = max(col[p][x], m[y][x][p]);
+        }
+    if (j.row_max) {
+#pragma unroll
+      for (int y = 0; y < DEEP; ++y) {
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) row[y] = max(row[y], uint32_t(__shfl_xor(int(row[y]), x, 64)));
+        if (lane == 0 && r0 + d + y < R) j.row_max[long(tc) * R + r0 + d + y] = row[y];
+      }
+    }
+  }
+  if (!j.col_max) return;
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+    for (int x = 0; x < NC; ++x) top[p][wave][x * 64 + lane] = col[p][x];
+  __syncthreads();
+  const int c = c0 + (tid & (kScanC - 1)), p = tid / kScanC, x = tid & (kScanC - 1);
+  if (c < C && p < PARTS)
+    j.col_max[(long(p) * ((R + kScanR - 1) / kScanR) + tr) * C + c] =
+        max(max(top[p][0][x], top[p][1][x]), max(top[p][2][x], top[p][3][x]));
+}
+
+__global__ __launch_bounds__(256) void k_scan(PackArgs a) {
+  __shared__ uint32_t top[2][4][kScanC];
+  int q = 0;
+#pragma unroll
+  for (int i = 1; i < kJobs; ++i)
+    if (i < a.jobs && int(blockIdx.x) >= a.job[i].scan0) q = i;
+  const PackJob& j = a.job[q];
+  const int id = int(blockIdx.x) - j.scan0, tr = id / j.scan_c, tc = id - tr * j.scan_c;
+  if (j.src) scan_tile<false>(j, a.s, tr, tc, top);
+  else scan_tile<true>(j, a.s, tr, tc, top);
+}
+
+// What the scan's tiles say together: the scale of every packed row, and its
+// count of small values from 0.  64 rows a workgroup, four shares of the tiles.
+struct ScaleJob {
+  const uint32_t* part;  // [parts][rows]
+  int parts, rows, block0;
+  Packed to;
+};
+constexpr int kScales = 6;
+struct ScaleArgs {
+  ScaleJob job[kScales];
+  int jobs;
+};
+constexpr int kNothing = -100000;  // the scale of a row of zeros
+__global__ __launch_bounds__(256) void k_scales(ScaleArgs a) {
+  __shared__ uint32_t top[256];
+  int q = 0;
+#pragma unroll
+  for (int i = 1; i < kScales; ++i)
+    if (i < a.jobs && int(blockIdx.x) >= a.job[i].block0) q = i;
+  const ScaleJob& j = a.job[q];
+  const int tid = threadIdx.x, r = (int(blockIdx.x) - j.block0) * 64 + (tid & 63), share = tid >> 6;
+  uint32_t m = 0;
+  if (r < j.rows)
+#pragma unroll 4
+    for (int p = share; p < j.parts; p += 4) m = max(m, j.part[long(p) * j.rows + r]);
+  top[tid] = m;
+  __syncthreads();
+  if (share || r >= (j.rows + 15) / 16 * 16) return;  // whole blocks: packed rows beyond the matrix are zeros
+  m = max(max(m, top[tid + 64]), max(top[tid + 128], top[tid + 192]));
+  const int at = ((r >> 4) * j.to.mul + j.to.add) * 16 + (r & 15);
+  const int e = m >> 23 ? int(m >> 23) - 127 : 31 - __clz(int(m)) - 149;
+  j.to.rows[at] = make_int2(m ? e - 14 : kNothing, 0);
+}
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// A lane's 8 values of a fragment, scaled and split.
 __device__ __forceinline__ void put_fragment(const Packed& to, int block, int step, int lane, const float (&v)[8]) {
-  Planes p;
-  split8<false>(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]}, p);
+  const int row = (block * to.mul + to.add) * 16 + (lane & 15), scale = to.rows[row].x;
+  f16x8 h, l;
+  int small = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = scale == kNothing ? 0.f : __builtin_ldexpf(v[i], -scale);
+    h[i] = _Float16(x);
+    l[i] = _Float16(x - float(h[i]));
+    small += fabsf(x) < 0.25f && v[i] != 0.f;
+  }
   char* at = to.p + (long(block * to.mul + to.add) * to.steps + step + to.first) * kFrag + lane * 16;
-  *reinterpret_cast<u32x4*>(at) = p.h;
-  *reinterpret_cast<u32x4*>(at + kPart) = p.m;
-  *reinterpret_cast<u32x4*>(at + 2 * kPart) = p.l;
+  *reinterpret_cast<f16x8*>(at) = h;
+  *reinterpret_cast<f16x8*>(at + kPart) = l;
+  small += __shfl_xor(small, 16, 64);
+  small += __shfl_xor(small, 32, 64);
+  if (small && lane < 16) atomicAdd(&to.rows[row].y, small);  // a count: any order gives the same
 }
 
 // A workgroup takes 32 x 64 values through LDS and writes them in both orders.
@@ -144,23 +290,30 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
   const int id = int(blockIdx.x) - j.block0, tr = id / j.tiles_c, tc = id - tr * j.tiles_c;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
   const int parts = j.src ? 1 : 2;
-  for (int i = tid; i < kPackR * kPackC; i += 256) {
-    const int r = i / kPackC, c = i % kPackC;
-    const long row = long(tr) * kPackR + r;
-    const int col = tc * kPackC + c;
-    const bool in = row < j.R && col < j.C;
-    const long at = row * j.C + col;
+  constexpr int EACH = kPackR * kPackC / 256;  // a thread's values, 4 rows apart, in flight together
+  const int c = tid % kPackC, col = tc * kPackC + c;
+  float v[3][EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const long row = long(tr) * kPackR + i * 4 + wave;
+    const long at = min(row, long(j.R - 1)) * j.C + min(col, j.C - 1);
+    v[0][i] = j.src ? j.src[at] : a.s.dh[at];
+    if (!j.src) {
+      v[1][i] = a.s.g[at];
+      v[2][i] = a.s.u[at];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int r = i * 4 + wave;
+    const bool in = tr * kPackR + r < j.R && col < j.C;
     if (j.src) {
-      tile[0][r * P + c] = in ? j.src[at] : 0.f;
+      tile[0][r * P + c] = in ? v[0][i] : 0.f;
     } else {
-      float s = 0.f, d = 0.f, act = 0.f, u = 0.f;
-      if (in) {
-        act = gate(a.s.act, a.s.g[at], &s);
-        d = a.s.dh[at];
-        u = a.s.u[at];
-      }
-      tile[0][r * P + c] = d * u * s;
-      tile[1][r * P + c] = d * act;
+      float slope;
+      const float act = gate(a.s.act, v[1][i], &slope);
+      tile[0][r * P + c] = in ? v[0][i] * v[2][i] * slope : 0.f;
+      tile[1][r * P + c] = in ? v[0][i] * act : 0.f;
     }
   }
   __syncthreads();
@@ -198,6 +351,7 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
 
 struct MmaArgs {
   const char *a, *b;  // packed operands
+  const int2 *rows_a, *rows_b;  // see Packed
   int product;
   int M, N;                  // rows of a and of b
   int steps, per;            // steps of 32 k, of a split
@@ -209,9 +363,6 @@ struct MmaArgs {
 };
 
 // Element (m, n) of a product goes where it belongs.
-struct Gated {
-  float g, u;
-};
 __device__ __forceinline__ void put_gated(const MmaArgs& a, long m, int c, float g, float u) {
   g += a.bg ? a.bg[c] : 0.f;
   u += a.bu ? a.bu[c] : 0.f;
@@ -227,6 +378,12 @@ __device__ __forceinline__ void put_gated(const MmaArgs& a, long m, int c, float
 typedef __attribute__((address_space(1))) const void gvoid;
 typedef __attribute__((address_space(3))) void lvoid;
 
+// Waits until at most N of this wavefront's loads are on their way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 // Tile id of the workgroup: the workgroups of an XCD (every eighth) take
 // neighbouring tiles, eight tile rows by the columns in turn, so that its L2
 // serves the operands that they share.
@@ -239,12 +396,20 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int* t
   *tn = in / high;
 }
 
+__device__ __forceinline__ f32x4 mfma_f16(f16x8 a, f16x8 b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Whether `small` values, each off by up to 2^-25 and multiplied by up to 2^15,
+// could show beside the largest sum of their row (or column) at 2^-22.
+__device__ __forceinline__ bool lossy(int small, float top) { return small && top < 4096.f * float(small); }
+
 // WM x WN wavefronts of FM x FN fragments of 16 x 16.
-template <int WM, int WN, int FM, int FN>
+template <int WM, int WN, int FM, int FN, int BUFS>
 __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaArgs a) {
-  constexpr int NW = WM * WN, TA = WM * FM, TB = WN * FN, LOADS = (TA + TB) * 3 / NW;
-  static_assert((TA + TB) * 3 % NW == 0, "whole fragments for every wavefront");
-  __shared__ __attribute__((aligned(16))) char lds[2][(TA + TB) * kFrag];
+  constexpr int NW = WM * WN, TA = WM * FM, TB = WN * FN, LOADS = (TA + TB) * kParts / NW;
+  static_assert((TA + TB) * kParts % NW == 0, "whole fragments for every wavefront");
+  __shared__ __attribute__((aligned(16))) char lds[BUFS][(TA + TB) * kFrag];
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
   int tm, tn;
@@ -252,13 +417,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaArgs a) {
   const int s0 = int(blockIdx.y) * a.per, s1 = min(a.steps, s0 + a.per);
   const long pitch = long(a.steps) * kFrag;
   // Part c of the tile's fragments: a's blocks first, then b's.
-  auto load = [&](int buf, int s) __attribute__((always_inline)) {
+  const char* from[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int c = wave * LOADS + i, f = c / kParts;
+    from[i] = (f < TA ? a.a + (long(tm) * TA + f) * pitch : a.b + (long(tn) * TB + f - TA) * pitch) +
+              long(s0) * kFrag + (c - f * kParts) * kPart;
+  }
+  auto load = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int c = wave * LOADS + i, f = c / 3;
-      const char* src = f < TA ? a.a + (long(tm) * TA + f) * pitch : a.b + (long(tn) * TB + f - TA) * pitch;
-      src += long(s) * kFrag + (c - f * 3) * kPart + lane * 16;
-      __builtin_amdgcn_global_load_lds((gvoid*)src, (lvoid*)(lds[buf] + c * kPart), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gvoid*)(from[i] + lane * 16), (lvoid*)(lds[buf] + (wave * LOADS + i) * kPart), 16, 0, 0);
+      from[i] += kFrag;
     }
   };
   f32x4 acc[FM][FN], low[FM][FN];
@@ -266,65 +436,112 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaArgs a) {
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  load(0, s0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the barrier alone does not wait for loads into LDS
-  __syncthreads();
-  for (int s = s0, buf = 0; s < s1; ++s, buf ^= 1) {
+  // One step of loads in flight for every buffer but one.  A barrier alone does
+  // not wait for loads into LDS: each wavefront waits for its own of the step
+  // at hand, and the barrier for everybody's; behind it the buffer of the step
+  // before is free.
+  constexpr int AHEAD = BUFS - 1;
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (s0 + i < s1) load(i);
+  for (int s = s0, buf = 0; s < s1; ++s, buf = buf == AHEAD ? 0 : buf + 1) {
+    if (AHEAD > 1 && s + 1 < s1) wait_loads<LOADS*(AHEAD - 1)>();
+    else wait_loads<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
     const char* A = lds[buf] + wm * FM * kFrag + lane * 16;
     const char* B = lds[buf] + (TA + wn * FN) * kFrag + lane * 16;
-    u32x4 pa[3][FM], pb[3][FN];
+    f16x8 pa[kParts][FM], pb[kParts][FN];
 #pragma unroll
-    for (int p = 0; p < 3; ++p) {
+    for (int p = 0; p < kParts; ++p) {
 #pragma unroll
-      for (int i = 0; i < FM; ++i) pa[p][i] = *reinterpret_cast<const u32x4*>(A + i * kFrag + p * kPart);
+      for (int i = 0; i < FM; ++i) pa[p][i] = *reinterpret_cast<const f16x8*>(A + i * kFrag + p * kPart);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) pb[p][j] = *reinterpret_cast<const u32x4*>(B + j * kFrag + p * kPart);
+      for (int j = 0; j < FN; ++j) pb[p][j] = *reinterpret_cast<const f16x8*>(B + j * kFrag + p * kPart);
     }
-    if (s + 1 < s1) load(buf ^ 1, s + 1);  // after the reads, which need not wait for it
-    // The products of the lower parts have sums of their own, so the main sum
-    // is rounded once per 32 k.
+    if (s + AHEAD < s1) load(buf == 0 ? AHEAD : buf - 1);  // after the reads, which need not wait for it
     auto mul = [&](f32x4 (&d)[FM][FN], int x, int y) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) d[i][j] = mfma_bf16(pa[x][i], pb[y][j], d[i][j]);
+        for (int j = 0; j < FN; ++j) d[i][j] = mfma_f16(pa[x][i], pb[y][j], d[i][j]);
     };
     mul(acc, 0, 0);
-    mul(low, 0, 1);
     mul(low, 1, 0);
-    mul(low, 1, 1);
-    mul(low, 0, 2);
-    mul(low, 2, 0);
-    __builtin_amdgcn_sched_barrier(0);  // the products first: they cover the loads
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    mul(low, 0, 1);
+    __builtin_amdgcn_sched_barrier(0);  // the products before the next wait: they cover the loads
   }
 
-  // Infinities, NaN and operands near the ends of the range do not survive
-  // the split (see split_gemm.hpp): such elements, and rows with no sum of
-  // kSplitTiny among the wavefront's columns, are formed again in FP32.  Each
-  // goes by its own row, so no row's bits depend on another row.
+  // Sums that are not finite, and rows and columns whose small values could
+  // show, are formed again in FP32, each by its own row or column.  A row (a
+  // column) is measured by its largest sum among the wavefront's.
   const long mw = (long(tm) * TA + wm * FM) * 16;
   const int nw = (tn * TB + wn * FN) * 16;
+  int2 ra[FM][4], rb[FN];
+  const int2 none = make_int2(kNothing, 0);
+  int small = 0;
   bool again = false;
-  uint32_t tiny = 0;  // bit 4 i + r: row r of fragments i
+#pragma unroll
+  for (int j = 0; j < FN; ++j) {
+    rb[j] = nw + j * 16 + lr < a.N ? a.rows_b[nw + j * 16 + lr] : none;
+    small |= rb[j].y;
+  }
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      float top = 0.f;
+      const long m = mw + i * 16 + 4 * lg + r;
+      ra[i][r] = m < a.M ? a.rows_a[m] : none;
+      small |= ra[i][r].y;
+    }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        float v = acc[i][j][r] += low[i][j][r];
-        if (mw + i * 16 + 4 * lg + r >= a.M || nw + j * 16 + lr >= a.N) v = 0.f;  // rows nobody packed
-        again = again || !__builtin_isfinite(v);
-        top = fmaxf(top, fabsf(v));
+        const bool in = ra[i][r].x != kNothing && rb[j].x != kNothing;  // else zeros, or a row nobody packed
+        acc[i][j][r] = in ? acc[i][j][r] + low[i][j][r] : 0.f;
+        again = again || !__builtin_isfinite(acc[i][j][r]);
+      }
+  uint32_t bad_a = 0, bad_b = 0;  // bit 4 i + r: row r of fragments i; bit j: this lane's column of fragments j
+  if (__any(small)) {
+    bool live_a = false, live_b = false;
+    float top_b[FN] = {};
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const float v = __builtin_isfinite(acc[i][j][r]) ? fabsf(acc[i][j][r]) : 0.f;
+          top = fmaxf(top, v);
+          top_b[j] = fmaxf(top_b[j], v);
+        }
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+        bad_a |= uint32_t(lossy(ra[i][r].y, top)) << (4 * i + r);
+        live_a = live_a || ra[i][r].x != kNothing;
       }
 #pragma unroll
-      for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-      tiny |= uint32_t(top > 0.f && top < kSplitTiny) << (4 * i + r);
+    for (int j = 0; j < FN; ++j) {
+      float top = fmaxf(top_b[j], __shfl_xor(top_b[j], 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      bad_b |= uint32_t(lossy(rb[j].y, top)) << j;
+      live_b = live_b || rb[j].x != kNothing;
     }
-  if (__any(again || tiny)) {
+    if (!__any(live_b)) bad_a = 0;  // beside zeros nothing shows
+    if (!__any(live_a)) bad_b = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j][r] = __builtin_ldexpf(acc[i][j][r], ra[i][r].x + rb[j].x);
+  if (__any(again || bad_a || bad_b)) {
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -347,7 +564,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaArgs a) {
       for (int j = 0; j < FN; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (!__builtin_isfinite(acc[i][j][r]) || (tiny >> (4 * i + r) & 1)) acc[i][j][r] = low[i][j][r];
+          if (!__builtin_isfinite(acc[i][j][r]) || (bad_a >> (4 * i + r) & 1) || (bad_b >> j & 1)) acc[i][j][r] = low[i][j][r];
   }
 
 #pragma unroll
@@ -439,7 +656,6 @@ struct FewArgs {
   MmaArgs out;
 };
 constexpr int kFewWaves = 8;
-__device__ __forceinline__ float at_or_zero(__amdgpu_buffer_rsrc_t r, uint32_t off) { return ld_f1(r, off); }
 
 template <int RB, bool XV>
 __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
@@ -468,8 +684,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const uint32_t off = in && k + r < K && n < N ? (uint32_t(k + r) * uint32_t(N) + uint32_t(n)) * 4u : ~0u;
-        w[0][d][r] = at_or_zero(rg, off);
-        w[1][d][r] = at_or_zero(ru, off);
+        w[0][d][r] = ld_f1(rg, off);
+        w[1][d][r] = ld_f1(ru, off);
       }
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
@@ -479,7 +695,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
         } else {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            x[d][b][r] = at_or_zero(rx, in && m < M && k + r < K ? (uint32_t(m) * uint32_t(K) + uint32_t(k + r)) * 4u : ~0u);
+            x[d][b][r] = ld_f1(rx, in && m < M && k + r < K ? (uint32_t(m) * uint32_t(K) + uint32_t(k + r)) * 4u : ~0u);
         }
       }
     }
@@ -520,7 +736,7 @@ long up_to(long n, long q) { return (n + q - 1) / q * q; }
 // Rows that read the weights as they are: beyond, packing them pays.
 constexpr int kFewRows = 32;
 
-// A product's tiles and splits: 128 x 128 where they fill the compute units
+// A product's tiles and splits: 256 x 128 where they fill the compute units
 // (or nearly), else 64 x 64, and k in splits while there are fewer workgroups
 // than two a compute unit and a split keeps kMinSteps steps.
 constexpr int kMinSteps = 6;
@@ -530,10 +746,10 @@ struct MmaPlan {
 };
 MmaPlan plan_mma(long M, long N, long steps) {
   MmaPlan p{};
-  p.big = ((M + 127) / 128) * ((N + 127) / 128) >= 192;
-  const int t = p.big ? 128 : 64;
-  p.tiles_m = int((M + t - 1) / t);
-  p.tiles_n = int((N + t - 1) / t);
+  p.big = ((M + 255) / 256) * ((N + 127) / 128) >= 192;
+  const int tm = p.big ? 256 : 64, tn = p.big ? 128 : 64;
+  p.tiles_m = int((M + tm - 1) / tm);
+  p.tiles_n = int((N + tn - 1) / tn);
   const long tiles = long(p.tiles_m) * p.tiles_n, want = p.big ? 256 : 512;
   long splits = tiles >= want / 2 ? 1 : std::min((want + tiles - 1) / tiles, std::max(1L, steps / kMinSteps));
   splits = std::min(splits, 64L);
@@ -542,9 +758,10 @@ MmaPlan plan_mma(long M, long N, long steps) {
   return p;
 }
 
-// One product: its packed operands and partial sums in the workspace.
+// One product: its packed operands with their scales, and its partial sums, in
+// the workspace.
 struct Layout {
-  long a, b, part;  // bytes
+  long a, b, rows, part;  // bytes
   MmaPlan plan;
   long rows_a, rows_b;
   int steps;
@@ -555,14 +772,32 @@ Layout layout_of(long M, long N, long steps) {
   l.rows_a = M;
   l.rows_b = N;
   l.steps = int(steps);
-  l.a = up_to(M, 128) / 16 * steps * kFrag;
+  l.a = up_to(M, 256) / 16 * steps * kFrag;  // whole tiles are read, whatever lies there
   l.b = up_to(N, 128) / 16 * steps * kFrag;
+  l.rows = up_to((up_to(M, 16) + up_to(N, 16)) * 8, 256);
   l.part = l.plan.splits > 1 ? up_to(long(l.plan.splits) * M * N * 4, 256) : 0;
   return l;
 }
+// The operands of a product laid out from `at`.
+struct Operands {
+  Packed a, b;
+};
+Operands operands_at(const Layout& l, char* at) {
+  int2* rows = reinterpret_cast<int2*>(at + l.a + l.b);
+  return Operands{Packed{at, l.steps, 0, 1, 0, rows}, Packed{at + l.a, l.steps, 0, 1, 0, rows + up_to(l.rows_a, 16)}};
+}
+Packed moved(Packed p, int first, int mul, int add) {
+  p.first = first;
+  p.mul = mul;
+  p.add = add;
+  return p;
+}
+long scan_rows(long R) { return (R + kScanR - 1) / kScanR; }
+long scan_cols(long C) { return (C + kScanC - 1) / kScanC; }
+
 struct Layouts {
   Layout fwd, dx, dw;
-  long sums;
+  long fwd_max, bwd_max, sums;  // bytes of the scans' results and of the column sums
 };
 Layouts layouts_of(const ttrl_gated_desc* d) {
   const long rows = std::max(1, d->M), both = up_to(d->N, 16) * 2, n32 = (d->N + 31) / 32;
@@ -570,6 +805,8 @@ Layouts layouts_of(const ttrl_gated_desc* d) {
   l.fwd = layout_of(rows, both, (d->K + 31) / 32);
   l.dx = layout_of(rows, d->K, 2 * n32);
   l.dw = layout_of(d->K, both, (rows + 31) / 32);
+  l.fwd_max = up_to((scan_cols(d->K) * rows + 2 * scan_rows(d->K) * d->N) * 4, 256);
+  l.bwd_max = up_to((scan_cols(d->N) * (rows + 2L * d->K) + scan_rows(rows) * (2L * d->N + d->K)) * 4, 256);
   l.sums = up_to((rows + 31) / 32 * 2 * d->N * 4, 256);
   return l;
 }
@@ -588,19 +825,34 @@ int check_gated(const ttrl_gated_desc* d, const char* name) {
   return TTRL_OK;
 }
 
-int launch_pack(ttrl_ctx* ctx, PackArgs& a, const char* name) {
-  long blocks = 0;
+int launch_pack(ttrl_ctx* ctx, PackArgs& a, ScaleArgs& c, const char* name) {
+  long blocks = 0, scans = 0, scales = 0;
   for (int i = 0; i < a.jobs; ++i) {
     PackJob& j = a.job[i];
     j.tiles_c = int((j.C + kPackC - 1) / kPackC);
     j.block0 = int(blocks);
     blocks += long(j.tiles_c) * ((j.R + kPackR - 1) / kPackR);
+    j.scan_c = int(scan_cols(j.C));
+    j.scan0 = int(scans);
+    scans += scan_cols(j.C) * scan_rows(j.R);
   }
+  for (int i = 0; i < c.jobs; ++i) {
+    c.job[i].block0 = int(scales);
+    scales += (c.job[i].rows + 63) / 64;
+  }
+  hipLaunchKernelGGL(k_scan, dim3(unsigned(scans)), dim3(256), 0, stream_of(ctx), a);
+  if (int rc = check_launch(name)) return rc;
+  hipLaunchKernelGGL(k_scales, dim3(unsigned(scales)), dim3(256), 0, stream_of(ctx), c);
+  if (int rc = check_launch(name)) return rc;
   hipLaunchKernelGGL(k_pack, dim3(unsigned(blocks)), dim3(256), 0, stream_of(ctx), a);
   return check_launch(name);
 }
 
-int launch_mma(ttrl_ctx* ctx, MmaArgs& a, const Layout& l, float* part, const char* name) {
+int launch_mma(ttrl_ctx* ctx, MmaArgs& a, const Layout& l, const Operands& o, float* part, const char* name) {
+  a.a = o.a.p;
+  a.b = o.b.p;
+  a.rows_a = o.a.rows;
+  a.rows_b = o.b.rows;
   a.M = int(l.rows_a);
   a.N = int(l.rows_b);
   a.steps = l.steps;
@@ -609,8 +861,8 @@ int launch_mma(ttrl_ctx* ctx, MmaArgs& a, const Layout& l, float* part, const ch
   a.tiles_n = l.plan.tiles_n;
   a.part = l.plan.splits > 1 ? part : nullptr;
   const dim3 grid(unsigned(a.tiles_m) * unsigned(a.tiles_n), unsigned(l.plan.splits));
-  if (l.plan.big) hipLaunchKernelGGL((k_mma<2, 2, 4, 4>), grid, dim3(256), 0, stream_of(ctx), a);
-  else hipLaunchKernelGGL((k_mma<2, 2, 2, 2>), grid, dim3(256), 0, stream_of(ctx), a);
+  if (l.plan.big) hipLaunchKernelGGL((k_mma<4, 2, 4, 4, 3>), grid, dim3(512), 0, stream_of(ctx), a);
+  else hipLaunchKernelGGL((k_mma<2, 2, 2, 2, 3>), grid, dim3(256), 0, stream_of(ctx), a);
   if (int rc = check_launch(name)) return rc;
   if (!a.part) return TTRL_OK;
   const long count = long(a.M) * (a.product == kInput ? a.N : a.s.N);
@@ -630,8 +882,9 @@ int ttrl_gated_space(const ttrl_gated_desc* d, long* forward_bytes, long* backwa
   if (int rc = check_gated(d, "ttrl_gated_space")) return rc;
   TTRL_REQUIRE(forward_bytes && backward_bytes, "ttrl_gated_space: null output");
   const Layouts l = layouts_of(d);
-  *forward_bytes = d->M <= kFewRows ? 0 : l.fwd.a + l.fwd.b + l.fwd.part;
-  *backward_bytes = l.dx.a + l.dx.b + l.dw.a + l.dw.b + std::max(l.dx.part, l.dw.part) + l.sums;
+  *forward_bytes = d->M <= kFewRows ? 0 : l.fwd.a + l.fwd.b + l.fwd.rows + l.fwd_max + l.fwd.part;
+  *backward_bytes = l.dx.a + l.dx.b + l.dx.rows + l.dw.a + l.dw.b + l.dw.rows + l.bwd_max +
+                    std::max(l.dx.part, l.dw.part) + l.sums;
   return TTRL_OK;
 }
 
@@ -664,21 +917,29 @@ int ttrl_gated_forward(ttrl_ctx* ctx, const ttrl_gated_desc* d) {
     return check_launch(name);
   }
   TTRL_REQUIRE(d->work && aligned16(d->work), "%s: null or unaligned workspace", name);
-  const Layout l = layouts_of(d).fwd;
-  char *pa = static_cast<char*>(d->work), *pb = pa + l.a;
+  const Layouts ls = layouts_of(d);
+  const Layout& l = ls.fwd;
+  char* at = static_cast<char*>(d->work);
+  const Operands o = operands_at(l, at);
+  uint32_t* tops = reinterpret_cast<uint32_t*>(at + l.a + l.b + l.rows);
   PackArgs p{};
+  ScaleArgs c{};
   p.s = m.s;
-  p.jobs = 3;
+  p.jobs = c.jobs = 3;
   p.job[0] = PackJob{d->x, d->M, d->K};
-  p.job[0].rows[0] = Packed{pa, l.steps, 0, 1, 0};
-  for (int q = 0; q < 2; ++q) {
-    p.job[1 + q] = PackJob{q ? d->w_up : d->w_gate, d->K, d->N};
-    p.job[1 + q].cols[0] = Packed{pb, l.steps, 0, 2, q};
+  p.job[0].rows[0] = o.a;
+  p.job[0].row_max = tops;
+  c.job[0] = ScaleJob{tops, int(scan_cols(d->K)), d->M, 0, o.a};
+  tops += scan_cols(d->K) * d->M;
+  for (int q = 0; q < 2; ++q, tops += scan_rows(d->K) * d->N) {
+    PackJob& w = p.job[1 + q];
+    w = PackJob{q ? d->w_up : d->w_gate, d->K, d->N};
+    w.cols[0] = moved(o.b, 0, 2, q);
+    w.col_max = tops;
+    c.job[1 + q] = ScaleJob{tops, int(scan_rows(d->K)), d->N, 0, w.cols[0]};
   }
-  if (int rc = launch_pack(ctx, p, name)) return rc;
-  m.a = pa;
-  m.b = pb;
-  return launch_mma(ctx, m, l, reinterpret_cast<float*>(pb + l.b), name);
+  if (int rc = launch_pack(ctx, p, c, name)) return rc;
+  return launch_mma(ctx, m, l, o, reinterpret_cast<float*>(at + l.a + l.b + l.rows + ls.fwd_max), name);
 }
 
 int ttrl_gated_backward(ttrl_ctx* ctx, const ttrl_gated_desc* d) {
@@ -701,52 +962,66 @@ int ttrl_gated_backward(ttrl_ctx* ctx, const ttrl_gated_desc* d) {
   TTRL_REQUIRE(d->work && aligned16(d->work), "%s: null or unaligned workspace", name);
   const Layouts l = layouts_of(d);
   const bool dw = d->dw_gate || d->dw_up, db = d->db_gate || d->db_up;
-  char *dxa = static_cast<char*>(d->work), *dxb = dxa + l.dx.a, *dwa = dxb + l.dx.b, *dwb = dwa + l.dw.a;
-  float* part = reinterpret_cast<float*>(dwb + l.dw.b);
-  float* sums = reinterpret_cast<float*>(dwb + l.dw.b + std::max(l.dx.part, l.dw.part));
+  if (!d->dx && !dw && !db) return TTRL_OK;
+  char *at_dx = static_cast<char*>(d->work), *at_dw = at_dx + l.dx.a + l.dx.b + l.dx.rows;
+  char* rest = at_dw + l.dw.a + l.dw.b + l.dw.rows;
+  const Operands odx = operands_at(l.dx, at_dx), odw = operands_at(l.dw, at_dw);
+  uint32_t* tops = reinterpret_cast<uint32_t*>(rest);
+  float* part = reinterpret_cast<float*>(rest + l.bwd_max);
+  float* sums = reinterpret_cast<float*>(rest + l.bwd_max + std::max(l.dx.part, l.dw.part));
   const int n32 = (d->N + 31) / 32;
   const Source s = source_of(d);
   PackArgs p{};
+  ScaleArgs c{};
   p.s = s;
+  auto scaled = [&](long parts, int rows, const Packed& to) {
+    c.job[c.jobs++] = ScaleJob{tops, int(parts), rows, 0, to};
+    uint32_t* at = tops;
+    tops += parts * rows;
+    return at;
+  };
   PackJob& slopes = p.job[p.jobs++];
   slopes = PackJob{nullptr, d->M, d->N};
   for (int q = 0; q < 2; ++q) {
-    if (d->dx) slopes.rows[q] = Packed{dxa, l.dx.steps, q * n32, 1, 0};
-    if (dw || db) slopes.cols[q] = Packed{dwb, l.dw.steps, 0, 2, q};
+    if (d->dx) slopes.rows[q] = moved(odx.a, q * n32, 1, 0);
+    if (dw || db) slopes.cols[q] = moved(odw.b, 0, 2, q);
+  }
+  if (d->dx) slopes.row_max = scaled(scan_cols(d->N), d->M, odx.a);  // both slopes are one row there
+  if (dw || db) {
+    slopes.col_max = scaled(scan_rows(d->M), d->N, slopes.cols[0]);
+    scaled(scan_rows(d->M), d->N, slopes.cols[1]);
   }
   slopes.sums = db ? sums : nullptr;
   if (dw) {
     PackJob& x = p.job[p.jobs++];
     x = PackJob{d->x, d->M, d->K};
-    x.cols[0] = Packed{dwa, l.dw.steps, 0, 1, 0};
+    x.cols[0] = odw.a;
+    x.col_max = scaled(scan_rows(d->M), d->K, odw.a);
   }
-  if (int rc = launch_pack(ctx, p, name)) return rc;
   if (d->dx) {
-    PackArgs w{};
-    w.s = s;
-    w.jobs = 2;
+    uint32_t* at = scaled(2 * scan_cols(d->N), d->K, odx.b);  // as are both weights
     for (int q = 0; q < 2; ++q) {
-      w.job[q] = PackJob{q ? d->w_up : d->w_gate, d->K, d->N};
-      w.job[q].rows[0] = Packed{dxb, l.dx.steps, q * n32, 1, 0};
+      PackJob& w = p.job[p.jobs++];
+      w = PackJob{q ? d->w_up : d->w_gate, d->K, d->N};
+      w.rows[0] = moved(odx.b, q * n32, 1, 0);
+      w.row_max = at + q * scan_cols(d->N) * d->K;
     }
-    if (int rc = launch_pack(ctx, w, name)) return rc;
+  }
+  if (int rc = launch_pack(ctx, p, c, name)) return rc;
+  if (d->dx) {
     MmaArgs m{};
-    m.a = dxa;
-    m.b = dxb;
     m.product = kInput;
     m.o0 = d->dx;
     m.s = s;
-    if (int rc = launch_mma(ctx, m, l.dx, part, name)) return rc;
+    if (int rc = launch_mma(ctx, m, l.dx, odx, part, name)) return rc;
   }
   if (dw) {
     MmaArgs m{};
-    m.a = dwa;
-    m.b = dwb;
     m.product = kWeight;
     m.o0 = d->dw_gate;
     m.o1 = d->dw_up;
     m.s = s;
-    if (int rc = launch_mma(ctx, m, l.dw, part, name)) return rc;
+    if (int rc = launch_mma(ctx, m, l.dw, odw, part, name)) return rc;
   }
   if (db) {
     hipLaunchKernelGGL(k_bias, dim3(ceil_div(2L * d->N, 16)), dim3(256), 0, stream_of(ctx), sums, (d->M + 31) / 32, d->N,
