@@ -204,3 +204,16 @@ def test_refusals(device):
             gated_linear(*bad)
     with pytest.raises(ValueError):
         gated_linear(t(2, 4), t(4, 5), t(4, 5), activation="tanh")
+
+
+@pytest.mark.parametrize("M", [70, 300])
+def test_small_values_beside_large_ones_that_meet_zeros(device, M):
+    """The largest value of every row of x, and of every row of the slopes,
+    meets a weight of zero, so all of the result comes from values 1e-7 of it
+    and less: the same bounds hold, in which the large ones have no part."""
+    x, dh = _inputs(11, M, 64, 48, False)
+    x["x"][:, 5] = 1e7
+    x["w_gate"][5] = x["w_up"][5] = 0
+    dh[:, 7] = 1e7
+    x["w_gate"][:, 7] = x["w_up"][:, 7] = 0
+    _check(_run(device, x, "sigmoid", dh), x, "sigmoid", dh)

@@ -47,7 +47,7 @@
 namespace ttrl {
 namespace {
 
-enum Act { kSilu, kGelu, kRelu, kSigmoid };
+enum Act { kSilu, kGelu, kRelu, kSigmoid, kNone };
 
 // act(g) and its derivative.
 __device__ __forceinline__ float gate(int act, float g, float* slope) {
@@ -132,7 +132,7 @@ struct PackJob {
   float* sums;                    // [R / 32][2][C] column sums of the slopes, or null
   int tiles_c, block0, scan_c, scan0;
 };
-constexpr int kJobs = 4, kPackR = 32, kPackC = 64, kScanR = 64, kScanC = 128;
+constexpr int kJobs = 4, kPackR = 32, kPackC = 64, kScanR = 32, kScanC = 128;
 struct PackArgs {
   PackJob job[kJobs];
   int jobs;
@@ -141,11 +141,12 @@ struct PackArgs {
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// The largest magnitudes of 64 x 128 values by row and by column.  NaN and
-// infinity count as the largest.  A wavefront has 16 rows, 8 (of slopes 4) of
-// them in flight.
-template <bool SLOPES>
+// The largest magnitudes of 32 x 128 values by row and by column.  NaN and
+// infinity count as the largest.  A wavefront has 8 rows, all (of slopes 4) in
+// flight.
+template <int ACT>  // of slopes; kNone: a plain matrix
 __device__ __forceinline__ void scan_tile(const PackJob& j, const Source& s, int tr, int tc, uint32_t (*top)[4][kScanC]) {
+  constexpr bool SLOPES = ACT != kNone;
   constexpr int NC = kScanC / 64, PARTS = SLOPES ? 2 : 1, DEEP = SLOPES ? 4 : 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int R = j.R, C = j.C, c0 = tc * kScanC, r0 = tr * kScanR + wave * (kScanR / 4);
@@ -173,7 +174,7 @@ __device__ __forceinline__ void scan_tile(const PackJob& j, const Source& s, int
       for (int x = 0; x < NC; ++x) {
         if constexpr (SLOPES) {
           float slope;
-          const float act = gate(s.act, v[0][y][x], &slope);
+          const float act = gate(ACT, v[0][y][x], &slope);
           m[y][x][0] = magnitude(v[2][y][x] * v[1][y][x] * slope);
           m[y][x][1] = magnitude(v[2][y][x] * act);
         } else {
@@ -218,8 +219,11 @@ __global__ __launch_bounds__(256) void k_scan(PackArgs a) {
     if (i < a.jobs && int(blockIdx.x) >= a.job[i].scan0) q = i;
   const PackJob& j = a.job[q];
   const int id = int(blockIdx.x) - j.scan0, tr = id / j.scan_c, tc = id - tr * j.scan_c;
-  if (j.src) scan_tile<false>(j, a.s, tr, tc, top);
-  else scan_tile<true>(j, a.s, tr, tc, top);
+  if (j.src) scan_tile<kNone>(j, a.s, tr, tc, top);
+  else if (a.s.act == kSilu) scan_tile<kSilu>(j, a.s, tr, tc, top);
+  else if (a.s.act == kGelu) scan_tile<kGelu>(j, a.s, tr, tc, top);
+  else if (a.s.act == kRelu) scan_tile<kRelu>(j, a.s, tr, tc, top);
+  else scan_tile<kSigmoid>(j, a.s, tr, tc, top);
 }
 
 // What the scan's tiles say together: the scale of every packed row, and its
@@ -259,8 +263,7 @@ __global__ __launch_bounds__(256) void k_scales(ScaleArgs a) {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // A lane's 8 values of a fragment, scaled and split.
-__device__ __forceinline__ void put_fragment(const Packed& to, int block, int step, int lane, const float (&v)[8]) {
-  const int row = (block * to.mul + to.add) * 16 + (lane & 15), scale = to.rows[row].x;
+__device__ __forceinline__ void put_fragment(const Packed& to, int block, int step, int lane, int scale, const float (&v)[8]) {
   f16x8 h, l;
   int small = 0;
 #pragma unroll
@@ -275,76 +278,93 @@ __device__ __forceinline__ void put_fragment(const Packed& to, int block, int st
   *reinterpret_cast<f16x8*>(at + kPart) = l;
   small += __shfl_xor(small, 16, 64);
   small += __shfl_xor(small, 32, 64);
-  if (small && lane < 16) atomicAdd(&to.rows[row].y, small);  // a count: any order gives the same
+  if (small && lane < 16) atomicAdd(&to.rows[(block * to.mul + to.add) * 16 + lane].y, small);  // a count: any order gives the same
 }
 
 // A workgroup takes 32 x 64 values through LDS and writes them in both orders.
+constexpr int kPackP = kPackC + 4;
+template <int ACT>
+__device__ __forceinline__ void pack_tile(const PackJob& j, const Source& s, int tr, int tc, float (*tile)[kPackR * kPackP]) {
+  constexpr bool SLOPES = ACT != kNone;
+  constexpr int P = kPackP, PARTS = SLOPES ? 2 : 1, EACH = kPackR * kPackC / 256;
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = tc * kPackC + lane;
+  // Four fragments each way: two blocks of 16 rows by two steps of columns,
+  // four blocks of 16 columns by one step of rows.
+  const int rb = tr * 2 + (wave >> 1), rs = tc * 2 + (wave & 1), cb = tc * 4 + wave;
+  const bool in_r = rb < (j.R + 15) / 16 && rs < (j.C + 31) / 32, in_c = cb < (j.C + 15) / 16;
+  int scale_r[PARTS] = {}, scale_c[PARTS] = {};
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    const Packed &r = j.rows[p], &k = j.cols[p];
+    if (r.p && in_r) scale_r[p] = r.rows[(rb * r.mul + r.add) * 16 + lr].x;
+    if (k.p && in_c) scale_c[p] = k.rows[(cb * k.mul + k.add) * 16 + lr].x;
+  }
+  float v[SLOPES ? 3 : 1][EACH];  // a thread's values, 4 rows apart, in flight together
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const long at = long(min(tr * kPackR + i * 4 + wave, j.R - 1)) * j.C + min(c, j.C - 1);
+    if constexpr (SLOPES) {
+      v[0][i] = s.g[at];
+      v[1][i] = s.u[at];
+      v[2][i] = s.dh[at];
+    } else {
+      v[0][i] = j.src[at];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int r = i * 4 + wave;
+    const bool in = tr * kPackR + r < j.R && c < j.C;
+    if constexpr (SLOPES) {
+      float slope;
+      const float act = gate(ACT, v[0][i], &slope);
+      tile[0][r * P + lane] = in ? v[2][i] * v[1][i] * slope : 0.f;
+      tile[1][r * P + lane] = in ? v[2][i] * act : 0.f;
+    } else {
+      tile[0][r * P + lane] = in ? v[0][i] : 0.f;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int part = 0; part < PARTS; ++part) {
+    const float* T = tile[part];
+    if (j.rows[part].p && in_r) {
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = T[((wave >> 1) * 16 + lr) * P + (wave & 1) * 32 + lg * 8 + i];
+      put_fragment(j.rows[part], rb, rs, lane, scale_r[part], w);
+    }
+    if (j.cols[part].p && in_c) {
+      float w[8], sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = T[(lg * 8 + i) * P + wave * 16 + lr];
+      put_fragment(j.cols[part], cb, tr, lane, scale_c[part], w);
+      if (SLOPES && j.sums) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += w[i];
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        const int col = tc * kPackC + wave * 16 + lr;
+        if (lg == 0 && col < j.C) j.sums[(long(tr) * 2 + part) * j.C + col] = sum;
+      }
+    }
+  }
+}
+
 __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
-  constexpr int P = kPackC + 4;
-  __shared__ __attribute__((aligned(16))) float tile[2][kPackR * P];
+  __shared__ __attribute__((aligned(16))) float tile[2][kPackR * kPackP];
   int q = 0;
 #pragma unroll
   for (int i = 1; i < kJobs; ++i)
     if (i < a.jobs && int(blockIdx.x) >= a.job[i].block0) q = i;
   const PackJob& j = a.job[q];
   const int id = int(blockIdx.x) - j.block0, tr = id / j.tiles_c, tc = id - tr * j.tiles_c;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
-  const int parts = j.src ? 1 : 2;
-  constexpr int EACH = kPackR * kPackC / 256;  // a thread's values, 4 rows apart, in flight together
-  const int c = tid % kPackC, col = tc * kPackC + c;
-  float v[3][EACH];
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const long row = long(tr) * kPackR + i * 4 + wave;
-    const long at = min(row, long(j.R - 1)) * j.C + min(col, j.C - 1);
-    v[0][i] = j.src ? j.src[at] : a.s.dh[at];
-    if (!j.src) {
-      v[1][i] = a.s.g[at];
-      v[2][i] = a.s.u[at];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const int r = i * 4 + wave;
-    const bool in = tr * kPackR + r < j.R && col < j.C;
-    if (j.src) {
-      tile[0][r * P + c] = in ? v[0][i] : 0.f;
-    } else {
-      float slope;
-      const float act = gate(a.s.act, v[1][i], &slope);
-      tile[0][r * P + c] = in ? v[0][i] * v[2][i] * slope : 0.f;
-      tile[1][r * P + c] = in ? v[0][i] * act : 0.f;
-    }
-  }
-  __syncthreads();
-  for (int part = 0; part < parts; ++part) {
-    const float* T = tile[part];
-    // Four fragments each way: two blocks of 16 rows by two steps of columns,
-    // four blocks of 16 columns by one step of rows.
-    if (j.rows[part].p) {
-      const int b = wave >> 1, s = wave & 1;
-      if (tr * 2 + b < (j.R + 15) / 16 && tc * 2 + s < (j.C + 31) / 32) {
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = T[(b * 16 + lr) * P + s * 32 + lg * 8 + i];
-        put_fragment(j.rows[part], tr * 2 + b, tc * 2 + s, lane, v);
-      }
-    }
-    if (j.cols[part].p && tc * 4 + wave < (j.C + 15) / 16) {
-      float v[8], sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = T[(lg * 8 + i) * P + wave * 16 + lr];
-      put_fragment(j.cols[part], tc * 4 + wave, tr, lane, v);
-      if (j.sums) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += v[i];
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        const int c = tc * kPackC + wave * 16 + lr;
-        if (lg == 0 && c < j.C) j.sums[(long(tr) * 2 + part) * j.C + c] = sum;
-      }
-    }
-  }
+  if (j.src) pack_tile<kNone>(j, a.s, tr, tc, tile);
+  else if (a.s.act == kSilu) pack_tile<kSilu>(j, a.s, tr, tc, tile);
+  else if (a.s.act == kGelu) pack_tile<kGelu>(j, a.s, tr, tc, tile);
+  else if (a.s.act == kRelu) pack_tile<kRelu>(j, a.s, tr, tc, tile);
+  else pack_tile<kSigmoid>(j, a.s, tr, tc, tile);
 }
 
 // ------------------------------------------------------------ the product ---
@@ -356,16 +376,15 @@ struct MmaArgs {
   int M, N;                  // rows of a and of b
   int steps, per;            // steps of 32 k, of a split
   int tiles_m, tiles_n;
+  bool wide;                 // results' rows start on 16 bytes
   float* part;               // partial sums of the splits, [split][M][N], or null
   const float *bg, *bu;      // kForward
   float *o0, *o1, *o2;       // kForward h, g, u; kInput dx; kWeight dW_gate, dW_up
   Source s;
 };
 
-// Element (m, n) of a product goes where it belongs.
+// Projections (biases added) of element (m, c) of h.
 __device__ __forceinline__ void put_gated(const MmaArgs& a, long m, int c, float g, float u) {
-  g += a.bg ? a.bg[c] : 0.f;
-  u += a.bu ? a.bu[c] : 0.f;
   const long at = m * a.s.N + c;
   float slope;
   a.o0[at] = gate(a.s.act, g, &slope) * u;
@@ -373,6 +392,19 @@ __device__ __forceinline__ void put_gated(const MmaArgs& a, long m, int c, float
     a.o1[at] = g;
     a.o2[at] = u;
   }
+}
+
+__device__ __forceinline__ float bias_of(const float* b, int c) { return b ? b[c] : 0.f; }
+
+// Columns c to c + 3 of a row of N.
+__device__ __forceinline__ void put4(float* row, int c, int N, bool wide, const f32x4& v) {
+  if (wide && c < N) {
+    *reinterpret_cast<f32x4*>(row + c) = v;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < N) row[c + e] = v[e];
 }
 
 typedef __attribute__((address_space(1))) const void gvoid;
@@ -445,7 +477,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaArgs a) {
   for (int i = 0; i < AHEAD; ++i)
     if (s0 + i < s1) load(i);
   for (int s = s0, buf = 0; s < s1; ++s, buf = buf == AHEAD ? 0 : buf + 1) {
-    if (AHEAD > 1 && s + 1 < s1) wait_loads<LOADS*(AHEAD - 1)>();
+    if (s + AHEAD - 1 < s1) wait_loads<LOADS*(AHEAD - 1)>();
     else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -473,133 +505,132 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaArgs a) {
     __builtin_amdgcn_sched_barrier(0);  // the products before the next wait: they cover the loads
   }
 
-  // Sums that are not finite, and rows and columns whose small values could
-  // show, are formed again in FP32, each by its own row or column.  A row (a
-  // column) is measured by its largest sum among the wavefront's.
+  // The rest by rows, through LDS, in loops that stay rolled: unrolled over the
+  // fragments it is more code than the instruction cache holds, and every
+  // workgroup waits for it (15 us and more).  Memory is written in whole lines.
+  constexpr int ROWS = FM * 16, COLS = FN * 16, PITCH = COLS + 4, L = COLS / 4;
+  static_assert(NW * ROWS * PITCH * 4 <= sizeof(lds), "the results fit in the buffers");
   const long mw = (long(tm) * TA + wm * FM) * 16;
   const int nw = (tn * TB + wn * FN) * 16;
-  int2 ra[FM][4], rb[FN];
+  __syncthreads();  // the buffers are read
+  float* mine = reinterpret_cast<float*>(&lds[0][0]) + wave * ROWS * PITCH;
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mine[(i * 16 + 4 * lg + r) * PITCH + j * 16 + lr] = acc[i][j][r] + low[i][j][r];
+
+  // Scales taken out.  Sums that are not finite, and rows and columns whose
+  // small values could show, are formed again in FP32, each by its own row or
+  // column, measured by its largest sum among the wavefront's.
   const int2 none = make_int2(kNothing, 0);
-  int small = 0;
-  bool again = false;
+  const int x4 = lane % L * 4, y0 = lane / L;
+  int2 rb[4];
+  float top_b[4] = {};
 #pragma unroll
-  for (int j = 0; j < FN; ++j) {
-    rb[j] = nw + j * 16 + lr < a.N ? a.rows_b[nw + j * 16 + lr] : none;
-    small |= rb[j].y;
-  }
+  for (int e = 0; e < 4; ++e) rb[e] = nw + x4 + e < a.N ? a.rows_b[nw + x4 + e] : none;
+  bool again = false, live_a = false;
+  uint32_t bad_a = 0;  // bit i: this lane's i-th row
+#pragma unroll 2
+  for (int i = 0; i < ROWS * L / 64; ++i) {
+    const int y = i * (64 / L) + y0;
+    const int2 ra = mw + y < a.M ? a.rows_a[mw + y] : none;
+    f32x4* at = reinterpret_cast<f32x4*>(mine + y * PITCH + x4);
+    f32x4 v = *at;
+    float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const long m = mw + i * 16 + 4 * lg + r;
-      ra[i][r] = m < a.M ? a.rows_a[m] : none;
-      small |= ra[i][r].y;
+    for (int e = 0; e < 4; ++e) {
+      if (ra.x == kNothing || rb[e].x == kNothing) v[e] = 0.f;  // and rows nobody packed
+      const bool fin = __builtin_isfinite(v[e]);
+      again = again || !fin;
+      const float size = fin ? fabsf(v[e]) : 0.f;
+      top = fmaxf(top, size);
+      top_b[e] = fmaxf(top_b[e], size);
+      v[e] = __builtin_ldexpf(v[e], ra.x + rb[e].x);
     }
+    *at = v;
+    live_a = live_a || ra.x != kNothing;
+    if (__any(ra.y)) {
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+      for (int x = 1; x < L; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+      bad_a |= uint32_t(lossy(ra.y, top)) << i;
+    }
+  }
+  bool bad_b[4], live_b = false, any_b = false;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+  for (int e = 0; e < 4; ++e) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const bool in = ra[i][r].x != kNothing && rb[j].x != kNothing;  // else zeros, or a row nobody packed
-        acc[i][j][r] = in ? acc[i][j][r] + low[i][j][r] : 0.f;
-        again = again || !__builtin_isfinite(acc[i][j][r]);
-      }
-  uint32_t bad_a = 0, bad_b = 0;  // bit 4 i + r: row r of fragments i; bit j: this lane's column of fragments j
-  if (__any(small)) {
-    bool live_a = false, live_b = false;
-    float top_b[FN] = {};
+    for (int x = L; x < 64; x <<= 1) top_b[e] = fmaxf(top_b[e], __shfl_xor(top_b[e], x, 64));
+    bad_b[e] = lossy(rb[e].y, top_b[e]);
+    any_b = any_b || bad_b[e];
+    live_b = live_b || rb[e].x != kNothing;
+  }
+  live_a = __any(live_a);
+  live_b = __any(live_b);  // beside zeros nothing shows
+  if (__any(again || (bad_a && live_b) || (any_b && live_a))) {
+#pragma unroll 1
+    for (int i = 0; i < ROWS * L / 64; ++i) {
+      float* at = mine + (i * (64 / L) + y0) * PITCH + x4;
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+      for (int e = 0; e < 4; ++e)
+        if ((live_b && (bad_a >> i & 1)) || (live_a && bad_b[e])) at[e] = __builtin_inff();
+    }
+#pragma unroll 1
+    for (int f = 0; f < FM * FN; ++f) {
+      const int i = f / FN, j = f % FN;
+      f32x4 exact = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int k = s0 * 32 + lg; k < s1 * 32 + lg; k += 4)
+        exact = mfma_f32(element_a(a.s, a.product, mw + i * 16 + lr, k), element_b(a.s, a.product, nw + j * 16 + lr, k), exact);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float top = 0.f;
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          const float v = __builtin_isfinite(acc[i][j][r]) ? fabsf(acc[i][j][r]) : 0.f;
-          top = fmaxf(top, v);
-          top_b[j] = fmaxf(top_b[j], v);
-        }
-#pragma unroll
-        for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-        bad_a |= uint32_t(lossy(ra[i][r].y, top)) << (4 * i + r);
-        live_a = live_a || ra[i][r].x != kNothing;
+        float* at = mine + (i * 16 + 4 * lg + r) * PITCH + j * 16 + lr;
+        if (!__builtin_isfinite(*at)) *at = exact[r];
       }
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      float top = fmaxf(top_b[j], __shfl_xor(top_b[j], 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      bad_b |= uint32_t(lossy(rb[j].y, top)) << j;
-      live_b = live_b || rb[j].x != kNothing;
     }
-    if (!__any(live_b)) bad_a = 0;  // beside zeros nothing shows
-    if (!__any(live_a)) bad_b = 0;
-  }
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j][r] = __builtin_ldexpf(acc[i][j][r], ra[i][r].x + rb[j].x);
-  if (__any(again || bad_a || bad_b)) {
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-      for (int j = 0; j < FN; ++j) low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-    for (int k = s0 * 32; k < s1 * 32; k += 4) {
-      float ea[FM], eb[FN];
-#pragma unroll
-      for (int i = 0; i < FM; ++i) ea[i] = element_a(a.s, a.product, mw + i * 16 + lr, k + lg);
-#pragma unroll
-      for (int j = 0; j < FN; ++j) eb[j] = element_b(a.s, a.product, nw + j * 16 + lr, k + lg);
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) low[i][j] = mfma_f32(ea[i], eb[j], low[i][j]);
-    }
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (!__builtin_isfinite(acc[i][j][r]) || (bad_a >> (4 * i + r) & 1) || (bad_b >> j & 1)) acc[i][j][r] = low[i][j][r];
   }
 
+  const bool sums = a.part || a.product == kInput;
+  if (sums) {
+    float* to = a.part ? a.part + long(blockIdx.y) * a.M * a.N : a.o0;
+#pragma unroll 2
+    for (int y = y0; y < ROWS; y += 64 / L)
+      if (mw + y < a.M) put4(to + (mw + y) * a.N, nw + x4, a.N, a.wide, *reinterpret_cast<const f32x4*>(mine + y * PITCH + x4));
+    return;
+  }
+  constexpr int H = L / 2;  // lanes to a row of either projection
+  const int x = lane % H * 4, at = (x >> 4) * 32 + (x & 15), c = nw / 2 + x, N = a.s.N;
+  f32x4 bg, bu;
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const long m = mw + i * 16 + 4 * lg + r;
-      if (m >= a.M) continue;
-      if (a.part) {
-        float* to = a.part + (long(blockIdx.y) * a.M + m) * a.N;
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          const int n = nw + j * 16 + lr;
-          if (n < a.N) to[n] = acc[i][j][r];
-        }
-      } else if (a.product == kInput) {
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          const int n = nw + j * 16 + lr;
-          if (n < a.N) a.o0[m * a.N + n] = acc[i][j][r];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < FN; j += 2) {
-          const int c = (nw + j * 16) / 2 + lr;
-          if (c >= a.s.N) continue;
-          if (a.product == kForward) {
-            put_gated(a, m, c, acc[i][j][r], acc[i][j + 1][r]);
-          } else {
-            if (a.o0) a.o0[m * a.s.N + c] = acc[i][j][r];
-            if (a.o1) a.o1[m * a.s.N + c] = acc[i][j + 1][r];
-          }
-        }
-      }
+  for (int e = 0; e < 4; ++e) {
+    bg[e] = bias_of(a.bg, min(c + e, N - 1));
+    bu[e] = bias_of(a.bu, min(c + e, N - 1));
+  }
+#pragma unroll 1
+  for (int y = lane / H; y < ROWS; y += 64 / H) {
+    if (mw + y >= a.M) break;
+    f32x4 g = *reinterpret_cast<const f32x4*>(mine + y * PITCH + at), u = *reinterpret_cast<const f32x4*>(mine + y * PITCH + at + 16);
+    const long row = (mw + y) * N;
+    if (a.product == kWeight) {
+      if (a.o0) put4(a.o0 + row, c, N, a.wide, g);
+      if (a.o1) put4(a.o1 + row, c, N, a.wide, u);
+      continue;
     }
+    f32x4 h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      g[e] += bg[e];
+      u[e] += bu[e];
+      float slope;
+      h[e] = gate(a.s.act, g[e], &slope) * u[e];
+    }
+    put4(a.o0 + row, c, N, a.wide, h);
+    if (a.o1) {
+      put4(a.o1 + row, c, N, a.wide, g);
+      put4(a.o2 + row, c, N, a.wide, u);
+    }
+  }
 }
 
 // The splits' sums, in order, and what follows them.
@@ -622,7 +653,7 @@ __global__ __launch_bounds__(256) void k_splits(MmaArgs a, int splits) {
       u += a.part[s * total + at + 16];
     }
     if (a.product == kForward) {
-      put_gated(a, m, c, g, u);
+      put_gated(a, m, c, g + bias_of(a.bg, c), u + bias_of(a.bu, c));
     } else {
       if (a.o0) a.o0[i] = g;
       if (a.o1) a.o1[i] = u;
@@ -724,7 +755,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
       g += part[w][i];
       u += part[w][RB * 256 + i];
     }
-    put_gated(a.out, m, c, g, u);
+    put_gated(a.out, m, c, g + bias_of(a.out.bg, c), u + bias_of(a.out.bu, c));
   }
 }
 
@@ -860,6 +891,8 @@ int launch_mma(ttrl_ctx* ctx, MmaArgs& a, const Layout& l, const Operands& o, fl
   a.tiles_m = l.plan.tiles_m;
   a.tiles_n = l.plan.tiles_n;
   a.part = l.plan.splits > 1 ? part : nullptr;
+  const int width = a.product == kInput || a.part ? a.N : a.s.N;
+  a.wide = width % 4 == 0 && (a.part || (aligned16(a.o0) && aligned16(a.o1) && aligned16(a.o2)));
   const dim3 grid(unsigned(a.tiles_m) * unsigned(a.tiles_n), unsigned(l.plan.splits));
   if (l.plan.big) hipLaunchKernelGGL((k_mma<4, 2, 4, 4, 3>), grid, dim3(512), 0, stream_of(ctx), a);
   else hipLaunchKernelGGL((k_mma<2, 2, 2, 2, 3>), grid, dim3(256), 0, stream_of(ctx), a);
