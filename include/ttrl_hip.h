@@ -928,7 +928,7 @@ int ttrl_gated_backward(ttrl_ctx* ctx, const ttrl_gated_desc* desc);
  * finite spoils its block.
  * counter: TTRL_ADAMW_COUNTER_BYTES of device memory, set by
  * ttrl_adamw_set_count (t updates done) and moved on by every step. */
-#define TTRL_ADAMW_COUNTER_BYTES 24
+#define TTRL_ADAMW_COUNTER_BYTES 2112
 typedef struct ttrl_adamw_tensor {
   float* p;
   const float* g;

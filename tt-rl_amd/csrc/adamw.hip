@@ -21,7 +21,7 @@
 //
 // One launch takes up to 64 tensors: their addresses travel in the kernel's
 // arguments, so the step can be captured into a graph and no table is uploaded.
-// A workgroup takes kSpan elements of one tensor, found by bisection over the
+// A workgroup takes one or four rounds of 1024 elements of one tensor, found by bisection over the
 // tensors' first workgroups.  Bound: HBM, 28 bytes a parameter in 32 bits,
 // 16.25 in 8 (4 + 4 + 4 of p and g, 2 + 2 of codes, 0.25 of scales).
 //
@@ -35,24 +35,41 @@
 namespace ttrl {
 namespace {
 
-constexpr int kThreads = 256, kRounds = 4, kSpan = kThreads * 4 * kRounds;
+constexpr int kThreads = 256, kRound = kThreads * 4;  // elements of a workgroup's round
+constexpr int kRounds = 4;
+constexpr long kMany = 1024;  // workgroups of kRounds rounds; below, one round each
 constexpr int kTensors = 64, kBlock = 64;
 
+// Tickets on one word cost 7 ns a workgroup, one after another, so workgroups
+// take them on one of kDesks lines, and a desk's last one on the first line.
+constexpr int kDesks = 32;
 struct Counter {
   int t;             // updates done
-  unsigned tickets;  // workgroups of the running launch that are done
+  unsigned tickets;  // desks of the running launch that are done
   double bc1, root;  // 1 - b1^(t+1) and 1 / sqrt(1 - b2^(t+1))
+  unsigned fill[10], desk[kDesks][16];
 };
 static_assert(sizeof(Counter) == TTRL_ADAMW_COUNTER_BYTES, "the size callers allocate");
 
+// b^n by squares: the same for a count that was set and one that was reached,
+// and short (pow() kept the last workgroup for 4 us).
+__device__ double power(double b, int n) {
+  double r = 1.0;
+  for (; n; n >>= 1, b *= b)
+    if (n & 1) r *= b;
+  return r;
+}
 __device__ void set_count(Counter* c, int t, double b1, double b2) {
   c->t = t;
   c->tickets = 0;
-  c->bc1 = 1.0 - pow(b1, double(t + 1));
-  c->root = 1.0 / sqrt(1.0 - pow(b2, double(t + 1)));
+  c->bc1 = 1.0 - power(b1, t + 1);
+  c->root = 1.0 / sqrt(1.0 - power(b2, t + 1));
 }
 
-__global__ void k_adamw_set(Counter* c, int t, double b1, double b2) { set_count(c, t, b1, b2); }
+__global__ void k_adamw_set(Counter* c, int t, double b1, double b2) {
+  c->desk[threadIdx.x][0] = 0;
+  if (threadIdx.x == 0) set_count(c, t, b1, b2);
+}
 
 struct Item {
   float* p;
@@ -125,6 +142,41 @@ __device__ __forceinline__ unsigned code_v(float v, float scale) {
   return unsigned(r > 0.f ? fmaxf(c, 1.f) : c);
 }
 
+// Four elements' codes.  Divided and rooted by the hardware's approximations (1
+// ulp each), x = 127 sqrt(r) is off by under 4e-5 and 255 r^(1/4) by under 8e-5
+// where scale and r are far from the range's ends, and the correctly rounded
+// forms above by as much: no half step within kSure means the same code.  The
+// rest (one of 20 wavefronts' rounds or so) takes the forms above.  They cost
+// two divisions and three roots an element, as much time as the memory:
+// @ADAMW@.
+constexpr float kSure = 2e-4f;
+__device__ __forceinline__ void codes4(const f32x4& m, const f32x4& v, float top_m, float top_v, uint32_t* cm, uint32_t* cv) {
+  auto usual = [](float s) { return s > 1e-30f && s < 1e30f; };
+  bool sure = usual(top_m) && usual(top_v);
+  const float im = __builtin_amdgcn_rcpf(top_m), iv = __builtin_amdgcn_rcpf(top_v);
+  uint32_t a = 0, b = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float x = __builtin_amdgcn_sqrtf(fabsf(m[j]) * im) * 127.f, r = v[j] * iv;
+    const float y = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(r)) * 255.f;
+    sure = sure && fabsf(__builtin_amdgcn_fractf(x) - 0.5f) > kSure && fabsf(__builtin_amdgcn_fractf(y) - 0.5f) > kSure &&
+           (r > 1e-30f || v[j] == 0.f);
+    const int c = int(rintf(x));
+    a |= (uint32_t(m[j] < 0.f ? -c : c) & 255u) << (8 * j);
+    b |= uint32_t(v[j] > 0.f ? fmaxf(rintf(y), 1.f) : 0.f) << (8 * j);
+  }
+  if (!sure) {
+    a = b = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a |= (uint32_t(code_m(m[j], top_m)) & 255u) << (8 * j);
+      b |= (code_v(v[j], top_v) & 255u) << (8 * j);
+    }
+  }
+  *cm = a;
+  *cv = b;
+}
+
 __device__ __forceinline__ int item_of(const AdamWArgs& a, int block) {
   int lo = 0, hi = a.count - 1;
   while (lo < hi) {
@@ -135,19 +187,19 @@ __device__ __forceinline__ int item_of(const AdamWArgs& a, int block) {
   return lo;
 }
 
-template <bool HELD>
+template <bool HELD, int ROUNDS>
 __global__ __launch_bounds__(kThreads) void k_adamw(AdamWArgs a) {
 #pragma clang fp contract(off)
   const Item& it = a.item[item_of(a, int(blockIdx.x))];
-  const long from = long(int(blockIdx.x) - it.first) * kSpan + threadIdx.x * 4, n = it.n;
+  const long from = long(int(blockIdx.x) - it.first) * (kRound * ROUNDS) + threadIdx.x * 4, n = it.n;
   const double bc1 = a.counter->bc1, root64 = a.counter->root;
-  f32x4 p[kRounds], g[kRounds], m[kRounds], v[kRounds];
-  uint32_t mc[kRounds], vc[kRounds];
-  float ms[kRounds], vs[kRounds];
-  bool in[kRounds], whole[kRounds];
+  f32x4 p[ROUNDS], g[ROUNDS], m[ROUNDS], v[ROUNDS];
+  uint32_t mc[ROUNDS], vc[ROUNDS];
+  float ms[ROUNDS], vs[ROUNDS];
+  bool in[ROUNDS], whole[ROUNDS];
 #pragma unroll
-  for (int u = 0; u < kRounds; ++u) {
-    const long i = from + u * (kThreads * 4), s = it.at + i;
+  for (int u = 0; u < ROUNDS; ++u) {
+    const long i = from + u * kRound, s = it.at + i;
     in[u] = i < n;
     whole[u] = it.wide && i + 4 <= n;
     if (!in[u]) continue;
@@ -165,8 +217,8 @@ __global__ __launch_bounds__(kThreads) void k_adamw(AdamWArgs a) {
   }
   const float size = float(a.lr / bc1), root = float(root64);
 #pragma unroll
-  for (int u = 0; u < kRounds; ++u) {
-    const long i = from + u * (kThreads * 4), s = it.at + i;
+  for (int u = 0; u < ROUNDS; ++u) {
+    const long i = from + u * kRound, s = it.at + i;
     float top_m = 0.f, top_v = 0.f;
     if (in[u]) {
 #pragma unroll
@@ -200,12 +252,8 @@ __global__ __launch_bounds__(kThreads) void k_adamw(AdamWArgs a) {
       top_m = row_max(top_m);
       top_v = row_max(top_v);
       if (in[u]) {
-        uint32_t cm = 0, cv = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          cm |= (uint32_t(code_m(m[u][j], top_m)) & 255u) << (8 * j);
-          cv |= (code_v(v[u][j], top_v) & 255u) << (8 * j);
-        }
+        uint32_t cm, cv;
+        codes4(m[u], v[u], top_m, top_v, &cm, &cv);
         *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + s) = cm;
         *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + s) = cv;
         if ((threadIdx.x & 15) == 0) {
@@ -218,7 +266,12 @@ __global__ __launch_bounds__(kThreads) void k_adamw(AdamWArgs a) {
   if (!a.last) return;
   // Every workgroup has read the corrections before it takes its ticket.
   __syncthreads();
-  if (threadIdx.x == 0 && atomicAdd(&a.counter->tickets, 1u) == gridDim.x - 1)
+  if (threadIdx.x) return;
+  const unsigned desk = blockIdx.x % kDesks, here = (gridDim.x - desk + kDesks - 1) / kDesks;
+  unsigned* tickets = a.counter->desk[desk];
+  if (atomicAdd(tickets, 1u) != here - 1) return;
+  *tickets = 0;
+  if (atomicAdd(&a.counter->tickets, 1u) == min(gridDim.x, unsigned(kDesks)) - 1)
     set_count(a.counter, a.counter->t + 1, a.b1d, a.b2d);
 }
 
@@ -235,6 +288,7 @@ struct HeldArgs {
 };
 
 // The values that the codes stand for.
+template <int ROUNDS>
 __global__ __launch_bounds__(kThreads) void k_adamw_held(HeldArgs a) {
   int lo = 0, hi = a.count - 1;
   while (lo < hi) {
@@ -243,10 +297,10 @@ __global__ __launch_bounds__(kThreads) void k_adamw_held(HeldArgs a) {
     else hi = mid - 1;
   }
   const HeldItem& it = a.item[lo];
-  const long from = long(int(blockIdx.x) - it.first) * kSpan + threadIdx.x * 4;
+  const long from = long(int(blockIdx.x) - it.first) * (kRound * ROUNDS) + threadIdx.x * 4;
 #pragma unroll
-  for (int u = 0; u < kRounds; ++u) {
-    const long i = from + u * (kThreads * 4), s = it.at + i;
+  for (int u = 0; u < ROUNDS; ++u) {
+    const long i = from + u * kRound, s = it.at + i;
     if (i >= it.n) continue;
     const uint32_t mc = *reinterpret_cast<const uint32_t*>(a.mc + s), vc = *reinterpret_cast<const uint32_t*>(a.vc + s);
     const float ms = a.ms[s / kBlock], vs = a.vs[s / kBlock];
@@ -262,7 +316,14 @@ __global__ __launch_bounds__(kThreads) void k_adamw_held(HeldArgs a) {
   }
 }
 
-int blocks_of(long n) { return int((n + kSpan - 1) / kSpan); }
+long blocks_of(long n, int rounds) { return (n + long(kRound) * rounds - 1) / (long(kRound) * rounds); }
+// Rounds of a workgroup: few elements are spread over the compute units (@ODD@).
+template <typename T>
+int rounds_of(const T* t, int count) {
+  long blocks = 0;
+  for (int i = 0; i < count; ++i) blocks += blocks_of(t[i].n, kRounds);
+  return blocks < kMany ? 1 : kRounds;
+}
 
 }  // namespace
 }  // namespace ttrl
@@ -275,7 +336,7 @@ int ttrl_adamw_set_count(ttrl_ctx* ctx, void* counter, int t, double beta1, doub
   TTRL_REQUIRE(ctx && counter, "ttrl_adamw_set_count: null argument");
   TTRL_REQUIRE(t >= 0 && beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0,
                "ttrl_adamw_set_count: t=%d, betas %g and %g", t, beta1, beta2);
-  hipLaunchKernelGGL(k_adamw_set, dim3(1), dim3(1), 0, stream_of(ctx), static_cast<Counter*>(counter), t, beta1, beta2);
+  hipLaunchKernelGGL(k_adamw_set, dim3(1), dim3(kDesks), 0, stream_of(ctx), static_cast<Counter*>(counter), t, beta1, beta2);
   return check_launch("ttrl_adamw_set_count");
 }
 
@@ -297,12 +358,13 @@ int ttrl_adamw_step(ttrl_ctx* ctx, int count, const ttrl_adamw_tensor* tensors, 
   for (int from = 0; from < count; from += kTensors) {
     AdamWArgs a{};
     a.count = std::min(kTensors, count - from);
+    const int rounds = rounds_of(tensors + from, a.count);
     long blocks = 0;
     for (int i = 0; i < a.count; ++i) {
       const ttrl_adamw_tensor& t = tensors[from + i];
       const bool wide = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g)) & 15) == 0;
       a.item[i] = {t.p, t.g, t.at, t.n, int(blocks), wide};
-      blocks += blocks_of(t.n);
+      blocks += blocks_of(t.n, rounds);
       TTRL_REQUIRE(blocks <= 0x7fffffffL, "%s: too many elements", name);
     }
     a.m = m;
@@ -320,8 +382,9 @@ int ttrl_adamw_step(ttrl_ctx* ctx, int count, const ttrl_adamw_tensor* tensors, 
     a.eps = float(eps);
     a.shrink = float(1.0 - lr * weight_decay);
     a.last = from + kTensors >= count;
-    if (state_bits == 8) hipLaunchKernelGGL(k_adamw<true>, dim3(unsigned(blocks)), dim3(kThreads), 0, stream_of(ctx), a);
-    else hipLaunchKernelGGL(k_adamw<false>, dim3(unsigned(blocks)), dim3(kThreads), 0, stream_of(ctx), a);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(kThreads), 0, stream_of(ctx), a); };
+    if (state_bits == 8) rounds == 1 ? go(k_adamw<true, 1>) : go(k_adamw<true, kRounds>);
+    else rounds == 1 ? go(k_adamw<false, 1>) : go(k_adamw<false, kRounds>);
     if (int rc = check_launch(name)) return rc;
   }
   return TTRL_OK;
@@ -339,18 +402,20 @@ int ttrl_adamw_moments(ttrl_ctx* ctx, int count, const ttrl_adamw_moment* tensor
   for (int from = 0; from < count; from += kTensors) {
     HeldArgs a{};
     a.count = std::min(kTensors, count - from);
+    const int rounds = rounds_of(tensors + from, a.count);
     long blocks = 0;
     for (int i = 0; i < a.count; ++i) {
       const ttrl_adamw_moment& t = tensors[from + i];
       a.item[i] = {t.m, t.v, t.at, t.n, int(blocks)};
-      blocks += blocks_of(t.n);
+      blocks += blocks_of(t.n, rounds);
       TTRL_REQUIRE(blocks <= 0x7fffffffL, "%s: too many elements", name);
     }
     a.mc = static_cast<const uint8_t*>(m);
     a.vc = static_cast<const uint8_t*>(v);
     a.ms = m_scale;
     a.vs = v_scale;
-    hipLaunchKernelGGL(k_adamw_held, dim3(unsigned(blocks)), dim3(kThreads), 0, stream_of(ctx), a);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(kThreads), 0, stream_of(ctx), a); };
+    rounds == 1 ? go(k_adamw_held<1>) : go(k_adamw_held<kRounds>);
     if (int rc = check_launch(name)) return rc;
   }
   return TTRL_OK;

@@ -161,7 +161,7 @@ class GatedDesc(C.Structure):
                                              "dw_gate", "dw_up", "db_gate", "db_up")])
 
 
-ADAMW_COUNTER_BYTES = 24
+ADAMW_COUNTER_BYTES = 2112
 
 
 class AdamWTensor(C.Structure):
