@@ -390,11 +390,10 @@ class AdamW(Optimizer):
         p = (1 - lr wd) p - (lr / bc1) m / (sqrt(v) / sqrt(bc2) + eps).
 
     `state_bits=8` holds both moments in a byte per element with a scale per
-    block of 64 (4.25 bytes of p's and the moments' 12 less in memory than
-    with 32): m to 1/127 of its block's largest near it and finer below
-    (steps of the square root), v in steps of the fourth root.  The update
-    count lives on the device, so a captured graph with the step replays
-    correctly."""
+    block of 64, 2.125 bytes a parameter in place of 8: m in 127 steps of the
+    square root either side of zero, v in 255 steps of the fourth root.  The
+    update count lives on the device, so a captured graph with the step
+    replays correctly."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
         super().__init__(params)
@@ -437,7 +436,10 @@ class AdamW(Optimizer):
         self.m, self.v = ([flat.view(at, p.shape) for at, p in zip(self.offsets, self.params)]
                           for flat in (self._m_flat, self._v_flat))
         self._counter = DeviceArray(dev, (_lib.ADAMW_COUNTER_BYTES,), np.uint8)
-        self._table, self._table_key = None, None
+        self._table = (_lib.AdamWTensor * len(self.params))(*[
+            (p.data.ptr, None, at, p.data.numel) for p, at in zip(self.params, self.offsets)])
+        self._out_table = (_lib.AdamWMoment * len(self.params))(*[
+            (None, None, at, p.data.numel) for p, at in zip(self.params, self.offsets)])
         self._set_count()
 
     def _set_count(self) -> None:
@@ -450,15 +452,11 @@ class AdamW(Optimizer):
             raise RuntimeError(f"AdamW.step: parameters {missing} hold no gradient for this step")
         settle(self.params)
         settle_sums(self.device)
-        key = [p.grad.ptr for p in self.params] + [p.data.ptr for p in self.params]
-        if key != self._table_key:
-            for i, p in enumerate(self.params):
-                if p.grad.numel != p.data.numel or p.grad.dtype != MASTER_DTYPE:
-                    raise ValueError(f"AdamW.step: parameter {i} has shape {p.shape}, its gradient {p.grad.shape} "
-                                     f"({p.grad.dtype})")
-            self._table = (_lib.AdamWTensor * len(self.params))(*[
-                (p.data.ptr, p.grad.ptr, at, p.data.numel) for p, at in zip(self.params, self.offsets)])
-            self._table_key = key
+        for i, (row, p) in enumerate(zip(self._table, self.params)):
+            g = p.grad
+            if g.numel != row.n or p.data.numel != row.n or g.dtype != MASTER_DTYPE:
+                raise ValueError(f"AdamW.step: parameter {i} has shape {p.shape}, its gradient {g.shape} ({g.dtype})")
+            row.p, row.g = p.data.ptr, g.ptr
         ms, vs = (a.vp for a in self._scales) if self._scales else (None, None)
         self.device.call("ttrl_adamw_step", len(self.params), self._table, self.state_bits, self._m_flat.vp,
                          self._v_flat.vp, ms, vs, self._counter.vp, self.lr, self.b1, self.b2, self.eps,
@@ -486,9 +484,9 @@ class AdamW(Optimizer):
             for dst, src in zip(out[0] + out[1], self.m + self.v):
                 dst.copy_from(src.reshape(dst.shape))
             return tuple(out)
-        table = (_lib.AdamWMoment * len(self.params))(*[
-            (m.ptr, v.ptr, at, p.data.numel) for m, v, at, p in zip(*out, self.offsets, self.params)])
-        self.device.call("ttrl_adamw_moments", len(self.params), table, self._m_flat.vp, self._v_flat.vp,
+        for row, m, v in zip(self._out_table, *out):
+            row.m, row.v = m.ptr, v.ptr
+        self.device.call("ttrl_adamw_moments", len(self.params), self._out_table, self._m_flat.vp, self._v_flat.vp,
                          *(a.vp for a in self._scales))
         return tuple(out)
 
