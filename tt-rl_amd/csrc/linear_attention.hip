@@ -263,7 +263,7 @@ __device__ __forceinline__ void pin(T& x) {
 
 // LOCAL: the first launch, what a segment adds to the state.
 template <int KP, int NW, bool VEC, bool LOCAL>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP == 128 ? 2 : 3))) void k_sweep(
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(KP >= 96 ? 2 : 3))) void k_sweep(
     SweepArgs a) {
   constexpr int NT = 64 * NW, KB = KP / 16, PX = KP + 4, PP = kChunk + 4;
   __shared__ __attribute__((aligned(16))) float lx[LOCAL ? 1 : 2][LOCAL ? 4 : kChunk * PX];
@@ -760,29 +760,47 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 bool wide(const Operand& o) { return !o.p || (o.dim % 4 == 0 && aligned16(o.p)); }
 
 template <bool LOCAL>
-int launch_sweeps(ttrl_ctx* ctx, const SweepArgs& a, int count, const char* name) {
-  int D = 0, E = 0;
+int launch_alike(ttrl_ctx* ctx, const SweepArgs& a, int count, int kp, int nw, const char* name) {
   bool vec = true;
-  for (int i = 0; i < count; ++i) {
-    D = std::max(D, a.s[i].x.dim);
-    E = std::max(E, a.s[i].z.dim);
-    vec = vec && wide(a.s[i].y) && (LOCAL || wide(a.s[i].x));
-  }
+  for (int i = 0; i < count; ++i) vec = vec && wide(a.s[i].y) && (LOCAL || wide(a.s[i].x));
   const dim3 grid(unsigned(a.B) * unsigned(a.H), unsigned((a.T + a.run - 1) / a.run), unsigned(count));
-  auto go = [&](auto kp, auto nw) {
-    constexpr int KP = decltype(kp)::value, NW = decltype(nw)::value;
+  auto go = [&](auto kpc, auto nwc) {
+    constexpr int KP = decltype(kpc)::value, NW = decltype(nwc)::value;
     if (vec) hipLaunchKernelGGL((k_sweep<KP, NW, true, LOCAL>), grid, dim3(64 * NW), 0, stream_of(ctx), a);
     else hipLaunchKernelGGL((k_sweep<KP, NW, false, LOCAL>), grid, dim3(64 * NW), 0, stream_of(ctx), a);
   };
-  auto width = [&](auto kp) {
-    if (decltype(kp)::value <= 64 && E <= 32) go(kp, std::integral_constant<int, decltype(kp)::value <= 64 ? 2 : 4>{});
-    else if (E <= 64) go(kp, std::integral_constant<int, 4>{});
-    else go(kp, std::integral_constant<int, 8>{});
+  auto width = [&](auto kpc) {
+    if (decltype(kpc)::value <= 64 && nw == 2) go(kpc, std::integral_constant<int, decltype(kpc)::value <= 64 ? 2 : 4>{});
+    else if (nw <= 4) go(kpc, std::integral_constant<int, 4>{});
+    else if (nw == 6) go(kpc, std::integral_constant<int, 6>{});
+    else go(kpc, std::integral_constant<int, 8>{});
   };
-  if (D <= 32) width(std::integral_constant<int, 32>{});
-  else if (D <= 64) width(std::integral_constant<int, 64>{});
+  if (kp == 32) width(std::integral_constant<int, 32>{});
+  else if (kp == 64) width(std::integral_constant<int, 64>{});
+  else if (kp == 96) width(std::integral_constant<int, 96>{});
   else width(std::integral_constant<int, 128>{});
   return check_launch(name);
+}
+
+// Sweeps of one shape go in one launch, others after them (head widths 40 and
+// 72: @SPLIT@).
+template <bool LOCAL>
+int launch_sweeps(ttrl_ctx* ctx, const SweepArgs& a, int count, const char* name) {
+  auto class_of = [](int n) { return (n + 31) / 32; };
+  bool gone[3] = {};
+  for (int i = 0; i < count; ++i) {
+    if (gone[i]) continue;
+    SweepArgs b = a;
+    const int kp = class_of(a.s[i].x.dim), nw = class_of(a.s[i].z.dim);
+    int same = 0;
+    for (int j = i; j < count; ++j)
+      if (class_of(a.s[j].x.dim) == kp && class_of(a.s[j].z.dim) == nw) {
+        b.s[same++] = a.s[j];
+        gone[j] = true;
+      }
+    if (int rc = launch_alike<LOCAL>(ctx, b, same, 32 * kp, 2 * nw, name)) return rc;
+  }
+  return TTRL_OK;
 }
 
 // Segments of whole chunks, kMark steps at most, and whether they run side by
