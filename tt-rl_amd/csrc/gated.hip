@@ -396,15 +396,75 @@ __device__ __forceinline__ void put_gated(const MmaArgs& a, long m, int c, float
 
 __device__ __forceinline__ float bias_of(const float* b, int c) { return b ? b[c] : 0.f; }
 
-// Columns c to c + 3 of a row of N.
-__device__ __forceinline__ void put4(float* row, int c, int N, bool wide, const f32x4& v) {
-  if (wide && c < N) {
-    *reinterpret_cast<f32x4*>(row + c) = v;
+// W columns of a row, on 16 bytes where W is 4.
+template <int W>
+__device__ __forceinline__ void put(float* to, const float (&v)[W]) {
+  if constexpr (W == 4) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+  else *to = v[0];
+}
+template <int W>
+__device__ __forceinline__ void get(const float* from, float (&v)[W]) {
+  if constexpr (W == 4) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(from);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = x[e];
+  } else {
+    v[0] = *from;
+  }
+}
+
+// A wavefront's results go from LDS where they belong, neighbouring lanes to
+// neighbouring columns, W at a time.
+template <int W, int ROWS, int COLS, int PITCH>
+__device__ __forceinline__ void put_tile(const MmaArgs& a, const float* mine, long m0, int n0, int lane) {
+  if (a.part || a.product == kInput) {
+    constexpr int L = COLS / W;  // lanes of a row
+    float* to = a.part ? a.part + long(blockIdx.y) * a.M * a.N : a.o0;
+    const int x = lane % L * W, n = n0 + x;
+    if (n >= a.N) return;
+#pragma unroll 2
+    for (int y = lane / L; y < ROWS; y += 64 / L) {
+      if (m0 + y >= a.M) break;
+      float v[W];
+      get(mine + y * PITCH + x, v);
+      put(to + (m0 + y) * a.N + n, v);
+    }
     return;
   }
+  constexpr int L = COLS / 2 / W;
+  const int x = lane % L * W, at = (x >> 4) * 32 + (x & 15), c = n0 / 2 + x, N = a.s.N;
+  if (c >= N) return;
+  float bg[W], bu[W];
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (c + e < N) row[c + e] = v[e];
+  for (int e = 0; e < W; ++e) {
+    bg[e] = bias_of(a.bg, c + e);
+    bu[e] = bias_of(a.bu, c + e);
+  }
+#pragma unroll 1
+  for (int y = lane / L; y < ROWS; y += 64 / L) {
+    if (m0 + y >= a.M) break;
+    float g[W], u[W], h[W];
+    get(mine + y * PITCH + at, g);
+    get(mine + y * PITCH + at + 16, u);
+    const long to = (m0 + y) * N + c;
+    if (a.product == kWeight) {
+      if (a.o0) put(a.o0 + to, g);
+      if (a.o1) put(a.o1 + to, u);
+      continue;
+    }
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      g[e] += bg[e];
+      u[e] += bu[e];
+      float slope;
+      h[e] = gate(a.s.act, g[e], &slope) * u[e];
+    }
+    put(a.o0 + to, h);
+    if (a.o1) {
+      put(a.o1 + to, g);
+      put(a.o2 + to, u);
+    }
+  }
 }
 
 typedef __attribute__((address_space(1))) const void gvoid;
@@ -524,18 +584,21 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaArgs a) {
   // Scales taken out.  Sums that are not finite, and rows and columns whose
   // small values could show, are formed again in FP32, each by its own row or
   // column, measured by its largest sum among the wavefront's.
-  const int2 none = make_int2(kNothing, 0);
   const int x4 = lane % L * 4, y0 = lane / L;
   int2 rb[4];
   float top_b[4] = {};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) rb[e] = nw + x4 + e < a.N ? a.rows_b[nw + x4 + e] : none;
+  for (int e = 0; e < 4; ++e) {
+    rb[e] = make_int2(kNothing, 0);
+    if (nw + x4 + e < a.N) rb[e] = a.rows_b[nw + x4 + e];
+  }
   bool again = false, live_a = false;
   uint32_t bad_a = 0;  // bit i: this lane's i-th row
 #pragma unroll 2
   for (int i = 0; i < ROWS * L / 64; ++i) {
     const int y = i * (64 / L) + y0;
-    const int2 ra = mw + y < a.M ? a.rows_a[mw + y] : none;
+    int2 ra = make_int2(kNothing, 0);
+    if (mw + y < a.M) ra = a.rows_a[mw + y];
     f32x4* at = reinterpret_cast<f32x4*>(mine + y * PITCH + x4);
     f32x4 v = *at;
     float top = 0.f;
@@ -591,46 +654,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaArgs a) {
     }
   }
 
-  const bool sums = a.part || a.product == kInput;
-  if (sums) {
-    float* to = a.part ? a.part + long(blockIdx.y) * a.M * a.N : a.o0;
-#pragma unroll 2
-    for (int y = y0; y < ROWS; y += 64 / L)
-      if (mw + y < a.M) put4(to + (mw + y) * a.N, nw + x4, a.N, a.wide, *reinterpret_cast<const f32x4*>(mine + y * PITCH + x4));
-    return;
-  }
-  constexpr int H = L / 2;  // lanes to a row of either projection
-  const int x = lane % H * 4, at = (x >> 4) * 32 + (x & 15), c = nw / 2 + x, N = a.s.N;
-  f32x4 bg, bu;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    bg[e] = bias_of(a.bg, min(c + e, N - 1));
-    bu[e] = bias_of(a.bu, min(c + e, N - 1));
-  }
-#pragma unroll 1
-  for (int y = lane / H; y < ROWS; y += 64 / H) {
-    if (mw + y >= a.M) break;
-    f32x4 g = *reinterpret_cast<const f32x4*>(mine + y * PITCH + at), u = *reinterpret_cast<const f32x4*>(mine + y * PITCH + at + 16);
-    const long row = (mw + y) * N;
-    if (a.product == kWeight) {
-      if (a.o0) put4(a.o0 + row, c, N, a.wide, g);
-      if (a.o1) put4(a.o1 + row, c, N, a.wide, u);
-      continue;
-    }
-    f32x4 h;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      g[e] += bg[e];
-      u[e] += bu[e];
-      float slope;
-      h[e] = gate(a.s.act, g[e], &slope) * u[e];
-    }
-    put4(a.o0 + row, c, N, a.wide, h);
-    if (a.o1) {
-      put4(a.o1 + row, c, N, a.wide, g);
-      put4(a.o2 + row, c, N, a.wide, u);
-    }
-  }
+  if (a.wide) put_tile<4, ROWS, COLS, PITCH>(a, mine, mw, nw, lane);
+  else put_tile<1, ROWS, COLS, PITCH>(a, mine, mw, nw, lane);
 }
 
 // The splits' sums, in order, and what follows them.
