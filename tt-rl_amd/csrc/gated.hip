@@ -375,12 +375,19 @@ struct MmaArgs {
   int product;
   int M, N;                  // rows of a and of b
   int steps, per;            // steps of 32 k, of a split
-  int tiles_m, tiles_n;
+  int tiles_m, tiles_n, splits;
   bool wide;                 // results' rows start on 16 bytes
   float* part;               // partial sums of the splits, [split][M][N], or null
   const float *bg, *bu;      // kForward
   float *o0, *o1, *o2;       // kForward h, g, u; kInput dx; kWeight dW_gate, dW_up
   Source s;
+};
+
+// Products of one launch: the second's workgroups start at a multiple of 8, so
+// that both go to the XCDs alike.
+struct MmaPair {
+  MmaArgs job[2];
+  int first;  // the second's first workgroup
 };
 
 // Projections (biases added) of element (m, c) of h.
@@ -416,10 +423,10 @@ __device__ __forceinline__ void get(const float* from, float (&v)[W]) {
 // A wavefront's results go from LDS where they belong, neighbouring lanes to
 // neighbouring columns, W at a time.
 template <int W, int ROWS, int COLS, int PITCH>
-__device__ __forceinline__ void put_tile(const MmaArgs& a, const float* mine, long m0, int n0, int lane) {
+__device__ __forceinline__ void put_tile(const MmaArgs& a, int split, const float* mine, long m0, int n0, int lane) {
   if (a.part || a.product == kInput) {
     constexpr int L = COLS / W;  // lanes of a row
-    float* to = a.part ? a.part + long(blockIdx.y) * a.M * a.N : a.o0;
+    float* to = a.part ? a.part + long(split) * a.M * a.N : a.o0;
     const int x = lane % L * W, n = n0 + x;
     if (n >= a.N) return;
 #pragma unroll 2
@@ -498,15 +505,19 @@ __device__ __forceinline__ bool lossy(int small, float top) { return small && to
 
 // WM x WN wavefronts of FM x FN fragments of 16 x 16.
 template <int WM, int WN, int FM, int FN, int BUFS>
-__global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaArgs a) {
+__global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
+  const int second = int(blockIdx.x) >= pair.first, id = int(blockIdx.x) - (second ? pair.first : 0);
+  const MmaArgs& a = pair.job[second];
+  const int tiles = a.tiles_m * a.tiles_n, split = id / tiles;
+  if (split >= a.splits) return;  // fills up to a multiple of 8
   constexpr int NW = WM * WN, TA = WM * FM, TB = WN * FN, LOADS = (TA + TB) * kParts / NW;
   static_assert((TA + TB) * kParts % NW == 0, "whole fragments for every wavefront");
   __shared__ __attribute__((aligned(16))) char lds[BUFS][(TA + TB) * kFrag];
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
   int tm, tn;
-  tile_of(int(blockIdx.x), a.tiles_m, a.tiles_n, &tm, &tn);
-  const int s0 = int(blockIdx.y) * a.per, s1 = min(a.steps, s0 + a.per);
+  tile_of(id - split * tiles, a.tiles_m, a.tiles_n, &tm, &tn);
+  const int s0 = split * a.per, s1 = min(a.steps, s0 + a.per);
   const long pitch = long(a.steps) * kFrag;
   // Part c of the tile's fragments: a's blocks first, then b's.
   const char* from[LOADS];
@@ -654,18 +665,26 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaArgs a) {
     }
   }
 
-  if (a.wide) put_tile<4, ROWS, COLS, PITCH>(a, mine, mw, nw, lane);
-  else put_tile<1, ROWS, COLS, PITCH>(a, mine, mw, nw, lane);
+  if (a.wide) put_tile<4, ROWS, COLS, PITCH>(a, split, mine, mw, nw, lane);
+  else put_tile<1, ROWS, COLS, PITCH>(a, split, mine, mw, nw, lane);
 }
 
-// The splits' sums, in order, and what follows them.
-__global__ __launch_bounds__(256) void k_splits(MmaArgs a, int splits) {
+// What follows the products: the splits' sums, in order, and the bias
+// gradients, the column sums of every 32 rows in order.
+struct FinishArgs {
+  MmaArgs job[2];
+  int blocks[2];  // workgroups of the products' splits; the rest sum columns
+  const float* sums;
+  int tiles, N;
+  float *db_gate, *db_up;
+};
+__device__ __forceinline__ void add_splits(const MmaArgs& a, int block, int blocks) {
   const long total = long(a.M) * a.N, half = long(a.M) * a.s.N;
   const long count = a.product == kInput ? total : half;
-  for (long i = long(blockIdx.x) * 256 + threadIdx.x; i < count; i += long(gridDim.x) * 256) {
+  for (long i = long(block) * 256 + threadIdx.x; i < count; i += long(blocks) * 256) {
     if (a.product == kInput) {
       float t = 0.f;
-      for (int s = 0; s < splits; ++s) t += a.part[s * total + i];
+      for (int s = 0; s < a.splits; ++s) t += a.part[s * total + i];
       a.o0[i] = t;
       continue;
     }
@@ -673,7 +692,7 @@ __global__ __launch_bounds__(256) void k_splits(MmaArgs a, int splits) {
     const int c = int(i - m * a.s.N);
     const long at = m * a.N + (c >> 4) * 32 + (c & 15);
     float g = 0.f, u = 0.f;
-    for (int s = 0; s < splits; ++s) {
+    for (int s = 0; s < a.splits; ++s) {
       g += a.part[s * total + at];
       u += a.part[s * total + at + 16];
     }
@@ -685,20 +704,25 @@ __global__ __launch_bounds__(256) void k_splits(MmaArgs a, int splits) {
     }
   }
 }
-
-// Bias gradients: the column sums of every 32 rows, in order.
-__global__ __launch_bounds__(256) void k_bias(const float* __restrict__ sums, int tiles, int N, float* __restrict__ db_gate,
-                                              float* __restrict__ db_up) {
+__global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
   __shared__ double red[256];
-  const int c = int(blockIdx.x) * 16 + (threadIdx.x & 15), q = threadIdx.x >> 4;
+  int block = int(blockIdx.x);
+  for (int j = 0; j < 2; ++j) {
+    if (block < a.blocks[j]) {
+      add_splits(a.job[j], block, a.blocks[j]);
+      return;
+    }
+    block -= a.blocks[j];
+  }
+  const int N = a.N, c = block * 16 + (threadIdx.x & 15), q = threadIdx.x >> 4;
   double t = 0.0;
   if (c < 2 * N)
-    for (int i = q; i < tiles; i += 16) t += double(sums[long(i) * 2 * N + c]);
+    for (int i = q; i < a.tiles; i += 16) t += double(a.sums[long(i) * 2 * N + c]);
   red[threadIdx.x] = t;
   __syncthreads();
   if (q || c >= 2 * N) return;
   for (int i = 1; i < 16; ++i) t += red[i * 16 + threadIdx.x];
-  float* to = c < N ? db_gate : db_up;
+  float* to = c < N ? a.db_gate : a.db_up;
   if (to) to[c < N ? c : c - N] = float(t);
 }
 
@@ -904,7 +928,7 @@ int launch_pack(ttrl_ctx* ctx, PackArgs& a, ScaleArgs& c, const char* name) {
   return check_launch(name);
 }
 
-int launch_mma(ttrl_ctx* ctx, MmaArgs& a, const Layout& l, const Operands& o, float* part, const char* name) {
+void fill_in(MmaArgs& a, const Layout& l, const Operands& o, float* part) {
   a.a = o.a.p;
   a.b = o.b.p;
   a.rows_a = o.a.rows;
@@ -915,17 +939,41 @@ int launch_mma(ttrl_ctx* ctx, MmaArgs& a, const Layout& l, const Operands& o, fl
   a.per = l.plan.per;
   a.tiles_m = l.plan.tiles_m;
   a.tiles_n = l.plan.tiles_n;
+  a.splits = l.plan.splits;
   a.part = l.plan.splits > 1 ? part : nullptr;
   const int width = a.product == kInput || a.part ? a.N : a.s.N;
   a.wide = width % 4 == 0 && (a.part || (aligned16(a.o0) && aligned16(a.o1) && aligned16(a.o2)));
-  const dim3 grid(unsigned(a.tiles_m) * unsigned(a.tiles_n), unsigned(l.plan.splits));
-  if (l.plan.big) hipLaunchKernelGGL((k_mma<4, 2, 4, 4, 3>), grid, dim3(512), 0, stream_of(ctx), a);
-  else hipLaunchKernelGGL((k_mma<2, 2, 2, 2, 3>), grid, dim3(256), 0, stream_of(ctx), a);
-  if (int rc = check_launch(name)) return rc;
-  if (!a.part) return TTRL_OK;
-  const long count = long(a.M) * (a.product == kInput ? a.N : a.s.N);
-  hipLaunchKernelGGL(k_splits, dim3(unsigned(std::min(2048L, (count + 255) / 256))), dim3(256), 0, stream_of(ctx), a,
-                     l.plan.splits);
+}
+
+// One or two products of one plan's tiles.
+int launch_mma(ttrl_ctx* ctx, const MmaArgs* const* jobs, int count, bool big, const char* name) {
+  MmaPair p{};
+  long blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    if (i) p.first = int(blocks = up_to(blocks, 8));
+    p.job[i] = *jobs[i];
+    blocks += long(jobs[i]->tiles_m) * jobs[i]->tiles_n * jobs[i]->splits;
+  }
+  if (count == 1) p.first = int(blocks);
+  const dim3 grid{unsigned(blocks)};
+  if (big) hipLaunchKernelGGL((k_mma<4, 2, 4, 4, 3>), grid, dim3(512), 0, stream_of(ctx), p);
+  else hipLaunchKernelGGL((k_mma<2, 2, 2, 2, 3>), grid, dim3(256), 0, stream_of(ctx), p);
+  return check_launch(name);
+}
+
+// Splits of the products that have any, and the bias gradients.
+int launch_finish(ttrl_ctx* ctx, const MmaArgs* const* jobs, int count, FinishArgs& a, const char* name) {
+  long blocks = a.sums ? ceil_div(2L * a.N, 16) : 0;
+  for (int i = 0; i < count; ++i) {
+    const MmaArgs& m = *jobs[i];
+    if (!m.part) continue;
+    a.job[i] = m;
+    const long n = long(m.M) * (m.product == kInput ? m.N : m.s.N);
+    a.blocks[i] = int(std::min(2048L, (n + 255) / 256));
+    blocks += a.blocks[i];
+  }
+  if (!blocks) return TTRL_OK;
+  hipLaunchKernelGGL(k_finish, dim3(unsigned(blocks)), dim3(256), 0, stream_of(ctx), a);
   return check_launch(name);
 }
 
@@ -942,7 +990,7 @@ int ttrl_gated_space(const ttrl_gated_desc* d, long* forward_bytes, long* backwa
   const Layouts l = layouts_of(d);
   *forward_bytes = d->M <= kFewRows ? 0 : l.fwd.a + l.fwd.b + l.fwd.rows + l.fwd_max + l.fwd.part;
   *backward_bytes = l.dx.a + l.dx.b + l.dx.rows + l.dw.a + l.dw.b + l.dw.rows + l.bwd_max +
-                    std::max(l.dx.part, l.dw.part) + l.sums;
+                    l.dx.part + l.dw.part + l.sums;
   return TTRL_OK;
 }
 
@@ -997,7 +1045,11 @@ int ttrl_gated_forward(ttrl_ctx* ctx, const ttrl_gated_desc* d) {
     c.job[1 + q] = ScaleJob{tops, int(scan_rows(d->K)), d->N, 0, w.cols[0]};
   }
   if (int rc = launch_pack(ctx, p, c, name)) return rc;
-  return launch_mma(ctx, m, l, o, reinterpret_cast<float*>(at + l.a + l.b + l.rows + ls.fwd_max), name);
+  fill_in(m, l, o, reinterpret_cast<float*>(at + l.a + l.b + l.rows + ls.fwd_max));
+  const MmaArgs* jobs[] = {&m};
+  if (int rc = launch_mma(ctx, jobs, 1, l.plan.big, name)) return rc;
+  FinishArgs f{};
+  return launch_finish(ctx, jobs, 1, f, name);
 }
 
 int ttrl_gated_backward(ttrl_ctx* ctx, const ttrl_gated_desc* d) {
@@ -1026,7 +1078,7 @@ int ttrl_gated_backward(ttrl_ctx* ctx, const ttrl_gated_desc* d) {
   const Operands odx = operands_at(l.dx, at_dx), odw = operands_at(l.dw, at_dw);
   uint32_t* tops = reinterpret_cast<uint32_t*>(rest);
   float* part = reinterpret_cast<float*>(rest + l.bwd_max);
-  float* sums = reinterpret_cast<float*>(rest + l.bwd_max + std::max(l.dx.part, l.dw.part));
+  float* sums = reinterpret_cast<float*>(rest + l.bwd_max + l.dx.part + l.dw.part);
   const int n32 = (d->N + 31) / 32;
   const Source s = source_of(d);
   PackArgs p{};
@@ -1066,27 +1118,32 @@ int ttrl_gated_backward(ttrl_ctx* ctx, const ttrl_gated_desc* d) {
     }
   }
   if (int rc = launch_pack(ctx, p, c, name)) return rc;
-  if (d->dx) {
-    MmaArgs m{};
-    m.product = kInput;
-    m.o0 = d->dx;
-    m.s = s;
-    if (int rc = launch_mma(ctx, m, l.dx, odx, part, name)) return rc;
+  MmaArgs mx{}, mw{};
+  mx.product = kInput;
+  mx.o0 = d->dx;
+  mw.product = kWeight;
+  mw.o0 = d->dw_gate;
+  mw.o1 = d->dw_up;
+  mx.s = mw.s = s;
+  fill_in(mx, l.dx, odx, part);
+  fill_in(mw, l.dw, odw, part + l.dx.part / 4);
+  const MmaArgs* jobs[2];
+  int count = 0;
+  if (d->dx) jobs[count++] = &mx;
+  if (dw) jobs[count++] = &mw;
+  if (count == 2 && l.dx.plan.big != l.dw.plan.big) {
+    if (int rc = launch_mma(ctx, jobs, 1, l.dx.plan.big, name)) return rc;
+    if (int rc = launch_mma(ctx, jobs + 1, 1, l.dw.plan.big, name)) return rc;
+  } else if (count) {
+    if (int rc = launch_mma(ctx, jobs, count, (d->dx ? l.dx : l.dw).plan.big, name)) return rc;
   }
-  if (dw) {
-    MmaArgs m{};
-    m.product = kWeight;
-    m.o0 = d->dw_gate;
-    m.o1 = d->dw_up;
-    m.s = s;
-    if (int rc = launch_mma(ctx, m, l.dw, odw, part, name)) return rc;
-  }
-  if (db) {
-    hipLaunchKernelGGL(k_bias, dim3(ceil_div(2L * d->N, 16)), dim3(256), 0, stream_of(ctx), sums, (d->M + 31) / 32, d->N,
-                       d->db_gate, d->db_up);
-    if (int rc = check_launch(name)) return rc;
-  }
-  return TTRL_OK;
+  FinishArgs f{};
+  f.sums = db ? sums : nullptr;
+  f.tiles = (d->M + 31) / 32;
+  f.N = d->N;
+  f.db_gate = d->db_gate;
+  f.db_up = d->db_up;
+  return launch_finish(ctx, jobs, count, f, name);
 }
 
 }  // extern "C"
