@@ -512,7 +512,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
   if (split >= a.splits) return;  // fills up to a multiple of 8
   constexpr int NW = WM * WN, TA = WM * FM, TB = WN * FN, LOADS = (TA + TB) * kParts / NW;
   static_assert((TA + TB) * kParts % NW == 0, "whole fragments for every wavefront");
-  __shared__ __attribute__((aligned(16))) char lds[BUFS][(TA + TB) * kFrag];
+  // The results leave through LDS, 64 columns of a wavefront at a time.
+  constexpr int ROWS = FM * 16, FH = FN < 4 ? FN : 4, COLS = FH * 16, PITCH = COLS + 4, L = COLS / 4;
+  constexpr int BUF = (TA + TB) * kFrag, OUT = NW * ROWS * PITCH * 4;
+  __shared__ __attribute__((aligned(16))) char lds[BUFS * BUF > OUT ? BUFS * BUF : OUT];
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
   int tm, tn;
@@ -530,15 +533,15 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
   auto load = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      __builtin_amdgcn_global_load_lds((gvoid*)(from[i] + lane * 16), (lvoid*)(lds[buf] + (wave * LOADS + i) * kPart), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gvoid*)(from[i] + lane * 16), (lvoid*)(lds + buf * BUF + (wave * LOADS + i) * kPart), 16, 0, 0);
       from[i] += kFrag;
     }
   };
-  f32x4 acc[FM][FN], low[FM][FN];
+  f32x4 acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   // One step of loads in flight for every buffer but one.  A barrier alone does
   // not wait for loads into LDS: each wavefront waits for its own of the step
   // at hand, and the barrier for everybody's; behind it the buffer of the step
@@ -553,8 +556,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    const char* A = lds[buf] + wm * FM * kFrag + lane * 16;
-    const char* B = lds[buf] + (TA + wn * FN) * kFrag + lane * 16;
+    const char* A = lds + buf * BUF + wm * FM * kFrag + lane * 16;
+    const char* B = lds + buf * BUF + (TA + wn * FN) * kFrag + lane * 16;
     f16x8 pa[kParts][FM], pb[kParts][FN];
 #pragma unroll
     for (int p = 0; p < kParts; ++p) {
@@ -564,33 +567,36 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
       for (int j = 0; j < FN; ++j) pb[p][j] = *reinterpret_cast<const f16x8*>(B + j * kFrag + p * kPart);
     }
     if (s + AHEAD < s1) load(buf == 0 ? AHEAD : buf - 1);  // after the reads, which need not wait for it
-    auto mul = [&](f32x4 (&d)[FM][FN], int x, int y) __attribute__((always_inline)) {
+    auto mul = [&](int x, int y) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) d[i][j] = mfma_f16(pa[x][i], pb[y][j], d[i][j]);
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma_f16(pa[x][i], pb[y][j], acc[i][j]);
     };
-    mul(acc, 0, 0);
-    mul(low, 1, 0);
-    mul(low, 0, 1);
+    mul(1, 0);
+    mul(0, 0);
+    mul(0, 1);
     __builtin_amdgcn_sched_barrier(0);  // the products before the next wait: they cover the loads
   }
 
   // The rest by rows, through LDS, in loops that stay rolled: unrolled over the
   // fragments it is more code than the instruction cache holds, and every
   // workgroup waits for it (15 us and more).  Memory is written in whole lines.
-  constexpr int ROWS = FM * 16, COLS = FN * 16, PITCH = COLS + 4, L = COLS / 4;
-  static_assert(NW * ROWS * PITCH * 4 <= sizeof(lds), "the results fit in the buffers");
   const long mw = (long(tm) * TA + wm * FM) * 16;
-  const int nw = (tn * TB + wn * FN) * 16;
   __syncthreads();  // the buffers are read
-  float* mine = reinterpret_cast<float*>(&lds[0][0]) + wave * ROWS * PITCH;
+  float* mine = reinterpret_cast<float*>(lds) + wave * ROWS * PITCH;
+#pragma unroll 1
+  for (int part = 0; part < FN / FH; ++part) {
+  const int nw = (tn * TB + wn * FN + part * FH) * 16;
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+  for (int x = 0; x < FN / FH; ++x)
+    if (part == x)
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
+      for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mine[(i * 16 + 4 * lg + r) * PITCH + j * 16 + lr] = acc[i][j][r] + low[i][j][r];
+        for (int j = 0; j < FH; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mine[(i * 16 + 4 * lg + r) * PITCH + j * 16 + lr] = acc[i][x * FH + j][r];
 
   // Scales taken out.  Sums that are not finite, and rows and columns whose
   // small values could show, are formed again in FP32, each by its own row or
@@ -651,8 +657,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
         if ((live_b && (bad_a >> i & 1)) || (live_a && bad_b[e])) at[e] = __builtin_inff();
     }
 #pragma unroll 1
-    for (int f = 0; f < FM * FN; ++f) {
-      const int i = f / FN, j = f % FN;
+    for (int f = 0; f < FM * FH; ++f) {
+      const int i = f / FH, j = f % FH;
       f32x4 exact = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
       for (int k = s0 * 32 + lg; k < s1 * 32 + lg; k += 4)
@@ -667,6 +673,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
 
   if (a.wide) put_tile<4, ROWS, COLS, PITCH>(a, split, mine, mw, nw, lane);
   else put_tile<1, ROWS, COLS, PITCH>(a, split, mine, mw, nw, lane);
+  }
 }
 
 // What follows the products: the splits' sums, in order, and the bias
@@ -824,13 +831,13 @@ struct MmaPlan {
   bool big;
   int tiles_m, tiles_n, splits, per;
 };
-MmaPlan plan_mma(long M, long N, long steps) {
+MmaPlan plan_mma(long M, long N, long steps, int together) {
   MmaPlan p{};
-  p.big = ((M + 255) / 256) * ((N + 127) / 128) >= 192;
-  const int tm = p.big ? 256 : 64, tn = p.big ? 128 : 64;
-  p.tiles_m = int((M + tm - 1) / tm);
-  p.tiles_n = int((N + tn - 1) / tn);
-  const long tiles = long(p.tiles_m) * p.tiles_n, want = p.big ? 256 : 512;
+  p.big = ((M + 255) / 256) * ((N + 255) / 256) * together >= 192;
+  const int t = p.big ? 256 : 64;
+  p.tiles_m = int((M + t - 1) / t);
+  p.tiles_n = int((N + t - 1) / t);
+  const long tiles = long(p.tiles_m) * p.tiles_n, want = p.big ? 256 / together : 512;
   long splits = tiles >= want / 2 ? 1 : std::min((want + tiles - 1) / tiles, std::max(1L, steps / kMinSteps));
   splits = std::min(splits, 64L);
   p.per = int((steps + splits - 1) / splits);
@@ -846,14 +853,14 @@ struct Layout {
   long rows_a, rows_b;
   int steps;
 };
-Layout layout_of(long M, long N, long steps) {
+Layout layout_of(long M, long N, long steps, int together) {
   Layout l{};
-  l.plan = plan_mma(M, N, steps);
+  l.plan = plan_mma(M, N, steps, together);
   l.rows_a = M;
   l.rows_b = N;
   l.steps = int(steps);
   l.a = up_to(M, 256) / 16 * steps * kFrag;  // whole tiles are read, whatever lies there
-  l.b = up_to(N, 128) / 16 * steps * kFrag;
+  l.b = up_to(N, 256) / 16 * steps * kFrag;
   l.rows = up_to((up_to(M, 16) + up_to(N, 16)) * 8, 256);
   l.part = l.plan.splits > 1 ? up_to(long(l.plan.splits) * M * N * 4, 256) : 0;
   return l;
@@ -882,9 +889,9 @@ struct Layouts {
 Layouts layouts_of(const ttrl_gated_desc* d) {
   const long rows = std::max(1, d->M), both = up_to(d->N, 16) * 2, n32 = (d->N + 31) / 32;
   Layouts l;
-  l.fwd = layout_of(rows, both, (d->K + 31) / 32);
-  l.dx = layout_of(rows, d->K, 2 * n32);
-  l.dw = layout_of(d->K, both, (rows + 31) / 32);
+  l.fwd = layout_of(rows, both, (d->K + 31) / 32, 1);
+  l.dx = layout_of(rows, d->K, 2 * n32, 2);
+  l.dw = layout_of(d->K, both, (rows + 31) / 32, 2);
   l.fwd_max = up_to((scan_cols(d->K) * rows + 2 * scan_rows(d->K) * d->N) * 4, 256);
   l.bwd_max = up_to((scan_cols(d->N) * (rows + 2L * d->K) + scan_rows(rows) * (2L * d->N + d->K)) * 4, 256);
   l.sums = up_to((rows + 31) / 32 * 2 * d->N * 4, 256);
@@ -956,7 +963,7 @@ int launch_mma(ttrl_ctx* ctx, const MmaArgs* const* jobs, int count, bool big, c
   }
   if (count == 1) p.first = int(blocks);
   const dim3 grid{unsigned(blocks)};
-  if (big) hipLaunchKernelGGL((k_mma<4, 2, 4, 4, 3>), grid, dim3(512), 0, stream_of(ctx), p);
+  if (big) hipLaunchKernelGGL((k_mma<4, 2, 4, 8, 2>), grid, dim3(512), 0, stream_of(ctx), p);
   else hipLaunchKernelGGL((k_mma<2, 2, 2, 2, 3>), grid, dim3(256), 0, stream_of(ctx), p);
   return check_launch(name);
 }
