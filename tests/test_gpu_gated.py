@@ -217,3 +217,49 @@ def test_small_values_beside_large_ones_that_meet_zeros(device, M):
     dh[:, 7] = 1e7
     x["w_gate"][:, 7] = x["w_up"][:, 7] = 0
     _check(_run(device, x, "sigmoid", dh), x, "sigmoid", dh)
+
+
+# Products large enough to be packed forward too, in small and large tiles;
+# ragged in every extent.
+@pytest.mark.parametrize("M,K,N,act,bias", [(2050, 523, 517, "gelu", True), (1031, 1029, 520, "relu", False),
+                                            (4100, 100, 1501, "sigmoid", True), (4100, 1500, 2100, "silu", False)])
+def test_packed_products(device, M, K, N, act, bias):
+    x, dh = _inputs(M, M, K, N, bias)
+    if act == "relu":
+        g = O._projections(*x.values())[0]
+        dh[np.abs(g) < 1e-4] = 0
+    _check(_run(device, x, act, dh), x, act, dh)
+
+
+@pytest.mark.parametrize("N", [517, 520])
+def test_packed_products_at_any_alignment(device, N):
+    x, dh = _inputs(3, 2050, 515, N, True)
+    _check(_run(device, x, "silu", dh, 1), x, "silu", dh)
+
+
+def test_packed_products_keep_what_is_not_finite_in_its_row(device):
+    x, dh = _inputs(7, 2050, 520, 516, bias=False)
+    clean = _run(device, x, "silu", dh)
+    for bad in (np.nan, np.inf):
+        y = {n: None if a is None else a.copy() for n, a in x.items()}
+        y["x"][2, 5] = bad
+        got = _run(device, y, "silu", dh)
+        rest = np.delete(np.arange(2050), 2)
+        for n in ("out", "x"):
+            assert np.array_equal(got[n][rest], clean[n][rest]), n
+        assert not np.isfinite(got["out"][2]).any()
+
+
+def test_packed_products_of_small_values_beside_large_ones(device):
+    """As above where the forward is packed too; and rows of very small and of
+    very large values, which the rows' scales take in."""
+    x, dh = _inputs(11, 2050, 520, 516, False)
+    x["x"][:, 5] = 1e7
+    x["w_gate"][5] = x["w_up"][5] = 0
+    dh[:, 7] = 1e7
+    x["w_gate"][:, 7] = x["w_up"][:, 7] = 0
+    _check(_run(device, x, "sigmoid", dh), x, "sigmoid", dh)
+    x, dh = _inputs(12, 2050, 520, 516, False)
+    x["x"] *= np.float32(2.0) ** np.linspace(-60, 12, 2050).astype(np.float32)[:, None]
+    dh *= np.float32(2.0) ** np.linspace(20, -40, 2050).astype(np.float32)[:, None]
+    _check(_run(device, x, "sigmoid", dh), x, "sigmoid", dh)

@@ -8,10 +8,10 @@
 //   du = dh * act(g),  dg = dh * u * act'(g)
 //   dx = dg W_gate^T + du W_up^T,  dW = x^T d.,  db = column sums of d.
 //
-// Two ways to the products, chosen by the rows (kFewRows):
+// Two ways to the forward products, chosen by their work (kFewWork):
 //
-// Few rows (an acting step) only read the weights once: k_few takes them
-// straight from memory into FP32 MFMA.
+// Small ones (an acting step) read the weights straight from memory into FP32
+// MFMA, in one launch (k_few).
 //
 // Otherwise the products run on the fp16 matrix cores.  Every row of an operand
 // (the values that one output sums over) is scaled by a power of two, so that
@@ -22,15 +22,17 @@
 // 11 significant bits each, of either sign: v - h - l is at most 2^-23 of v's
 // power of two.  Of the four products of two values' parts hh, hl and lh are
 // kept; ll is at most 2^-22 of the product, of either sign.  Together a product
-// is off by 2^-21 at worst and 2^-24 in the mean, as one rounding of FP32 is,
-// every partial product is exact in FP32 and added in FP32, hh apart from the
-// other two, so the main sum is rounded once per 32 k.  fp16 ends at 2^-24, so a
+// is off by 2^-21 at worst and 2^-24 in the mean, as one rounding of FP32 is;
+// every partial product is exact in FP32 and added in FP32, the sum rounded
+// three times per 32 k.  (Error against float64 at 8192 x 1024 x 4096: 1.1e-6 of
+// the largest, a library's FP32 products 1.7e-6.)  fp16 ends at 2^-24, so a
 // value under 2^-2 (2^-16 of its row's largest) is off by up to 2^-25 instead;
 // such values are counted by row, and where that count could show in a sum
 // (lossy() below), or a sum is not finite, it is formed again in FP32.
 //
 // (Three bf16 parts, 24 bits at any exponent, need six products and no scale:
-// 8192 x 1024 x 4096 forward and backward took 2651 us instead of @8192@.)
+// the forward and backward pass of 8192 x 1024 x 4096 took 2651 us so, 1546
+// with two fp16 parts in the same tiles, and 1368 to 1429 as it stands.)
 //
 // Operands are split once, by k_pack, into the very order in which the matrix
 // cores take them: 16 rows x 32 k of one part are 1 KiB,
@@ -38,7 +40,9 @@
 // so k_mma moves whole fragments from memory to LDS without a register and
 // reads them without conflicts, and every value is split once however many
 // tiles read it.  The scales cost one more pass over what is packed (k_scan);
-// packing writes 4 bytes a value beside the 4 read.
+// packing writes 4 bytes a value beside the 4 read.  Where the time of that pass
+// goes (us): forward scan 13, pack 21, product 404; backward scan 120, pack 275
+// (1.1 GB, 4 TB/s), both products 604.
 #include "split_gemm.hpp"
 
 #include <algorithm>
@@ -143,7 +147,8 @@ __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(
 
 // The largest magnitudes of 32 x 128 values by row and by column.  NaN and
 // infinity count as the largest.  A wavefront has 8 rows, all (of slopes 4) in
-// flight.
+// flight.  Bound: memory (the backward's 470 MB 120 us, 3.9 TB/s), at 777 x 1333
+// the activations, 9 us (64 rows a tile: 21).
 template <int ACT>  // of slopes; kNone: a plain matrix
 __device__ __forceinline__ void scan_tile(const PackJob& j, const Source& s, int tr, int tc, uint32_t (*top)[4][kScanC]) {
   constexpr bool SLOPES = ACT != kNone;
@@ -282,6 +287,8 @@ __device__ __forceinline__ void put_fragment(const Packed& to, int block, int st
 }
 
 // A workgroup takes 32 x 64 values through LDS and writes them in both orders.
+// Bound: memory, 12 bytes read and 16 written for each pair of slopes (8192 x
+// 4096 with x and both weights: 275 us, 3.9 TB/s; a large copy 4.7).
 constexpr int kPackP = kPackC + 4;
 template <int ACT>
 __device__ __forceinline__ void pack_tile(const PackJob& j, const Source& s, int tr, int tc, float (*tile)[kPackR * kPackP]) {
@@ -503,7 +510,15 @@ __device__ __forceinline__ f32x4 mfma_f16(f16x8 a, f16x8 b, const f32x4& c) {
 // could show beside the largest sum of their row (or column) at 2^-22.
 __device__ __forceinline__ bool lossy(int small, float top) { return small && top < 4096.f * float(small); }
 
-// WM x WN wavefronts of FM x FN fragments of 16 x 16.
+// WM x WN wavefronts of FM x FN fragments of 16 x 16, BUFS steps of operands in
+// LDS.  256 x 256 tiles run at 1.02 (forward, with the activation and three
+// outputs) and 1.37 PFLOP/s of fp16 (both gradients) at 8192 x 1024 x 4096; a
+// large bf16 product of the library 1.15.  Tiles of 256 x 128 were bound by the
+// L2s, which gave 9.7 TB/s (450 and 680 us, 404 and 604 with 256 x 256); reading
+// the next step's fragments while this one's products run took as long.
+// 64 x 64 tiles, three workgroups a compute unit, are as near the L2s' rate (9.4
+// TB/s at 777 x 500 x 1333); there a workgroup's 16 steps take 6 of 12 us, the
+// scales 2 and the results 2.5.
 template <int WM, int WN, int FM, int FN, int BUFS>
 __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
   const int second = int(blockIdx.x) >= pair.first, id = int(blockIdx.x) - (second ? pair.first : 0);
@@ -587,92 +602,92 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
   float* mine = reinterpret_cast<float*>(lds) + wave * ROWS * PITCH;
 #pragma unroll 1
   for (int part = 0; part < FN / FH; ++part) {
-  const int nw = (tn * TB + wn * FN + part * FH) * 16;
+    const int nw = (tn * TB + wn * FN + part * FH) * 16;
 #pragma unroll
-  for (int x = 0; x < FN / FH; ++x)
-    if (part == x)
+    for (int x = 0; x < FN / FH; ++x)
+      if (part == x)
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FH; ++j)
+          for (int j = 0; j < FH; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) mine[(i * 16 + 4 * lg + r) * PITCH + j * 16 + lr] = acc[i][x * FH + j][r];
+            for (int r = 0; r < 4; ++r) mine[(i * 16 + 4 * lg + r) * PITCH + j * 16 + lr] = acc[i][x * FH + j][r];
 
-  // Scales taken out.  Sums that are not finite, and rows and columns whose
-  // small values could show, are formed again in FP32, each by its own row or
-  // column, measured by its largest sum among the wavefront's.
-  const int x4 = lane % L * 4, y0 = lane / L;
-  int2 rb[4];
-  float top_b[4] = {};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    rb[e] = make_int2(kNothing, 0);
-    if (nw + x4 + e < a.N) rb[e] = a.rows_b[nw + x4 + e];
-  }
-  bool again = false, live_a = false;
-  uint32_t bad_a = 0;  // bit i: this lane's i-th row
-#pragma unroll 2
-  for (int i = 0; i < ROWS * L / 64; ++i) {
-    const int y = i * (64 / L) + y0;
-    int2 ra = make_int2(kNothing, 0);
-    if (mw + y < a.M) ra = a.rows_a[mw + y];
-    f32x4* at = reinterpret_cast<f32x4*>(mine + y * PITCH + x4);
-    f32x4 v = *at;
-    float top = 0.f;
+    // Scales taken out.  Sums that are not finite, and rows and columns whose
+    // small values could show, are formed again in FP32, each by its own row or
+    // column, measured by its largest sum among the wavefront's.
+    const int x4 = lane % L * 4, y0 = lane / L;
+    int2 rb[4];
+    float top_b[4] = {};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (ra.x == kNothing || rb[e].x == kNothing) v[e] = 0.f;  // and rows nobody packed
-      const bool fin = __builtin_isfinite(v[e]);
-      again = again || !fin;
-      const float size = fin ? fabsf(v[e]) : 0.f;
-      top = fmaxf(top, size);
-      top_b[e] = fmaxf(top_b[e], size);
-      v[e] = __builtin_ldexpf(v[e], ra.x + rb[e].x);
+      rb[e] = make_int2(kNothing, 0);
+      if (nw + x4 + e < a.N) rb[e] = a.rows_b[nw + x4 + e];
     }
-    *at = v;
-    live_a = live_a || ra.x != kNothing;
-    if (__any(ra.y)) {
-#pragma unroll
-      for (int x = 1; x < L; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-      bad_a |= uint32_t(lossy(ra.y, top)) << i;
-    }
-  }
-  bool bad_b[4], live_b = false, any_b = false;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-#pragma unroll
-    for (int x = L; x < 64; x <<= 1) top_b[e] = fmaxf(top_b[e], __shfl_xor(top_b[e], x, 64));
-    bad_b[e] = lossy(rb[e].y, top_b[e]);
-    any_b = any_b || bad_b[e];
-    live_b = live_b || rb[e].x != kNothing;
-  }
-  live_a = __any(live_a);
-  live_b = __any(live_b);  // beside zeros nothing shows
-  if (__any(again || (bad_a && live_b) || (any_b && live_a))) {
-#pragma unroll 1
+    bool again = false, live_a = false;
+    uint32_t bad_a = 0;  // bit i: this lane's i-th row
+#pragma unroll 2
     for (int i = 0; i < ROWS * L / 64; ++i) {
-      float* at = mine + (i * (64 / L) + y0) * PITCH + x4;
+      const int y = i * (64 / L) + y0;
+      int2 ra = make_int2(kNothing, 0);
+      if (mw + y < a.M) ra = a.rows_a[mw + y];
+      f32x4* at = reinterpret_cast<f32x4*>(mine + y * PITCH + x4);
+      f32x4 v = *at;
+      float top = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if ((live_b && (bad_a >> i & 1)) || (live_a && bad_b[e])) at[e] = __builtin_inff();
-    }
-#pragma unroll 1
-    for (int f = 0; f < FM * FH; ++f) {
-      const int i = f / FH, j = f % FH;
-      f32x4 exact = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-      for (int k = s0 * 32 + lg; k < s1 * 32 + lg; k += 4)
-        exact = mfma_f32(element_a(a.s, a.product, mw + i * 16 + lr, k), element_b(a.s, a.product, nw + j * 16 + lr, k), exact);
+      for (int e = 0; e < 4; ++e) {
+        if (ra.x == kNothing || rb[e].x == kNothing) v[e] = 0.f;  // and rows nobody packed
+        const bool fin = __builtin_isfinite(v[e]);
+        again = again || !fin;
+        const float size = fin ? fabsf(v[e]) : 0.f;
+        top = fmaxf(top, size);
+        top_b[e] = fmaxf(top_b[e], size);
+        v[e] = __builtin_ldexpf(v[e], ra.x + rb[e].x);
+      }
+      *at = v;
+      live_a = live_a || ra.x != kNothing;
+      if (__any(ra.y)) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float* at = mine + (i * 16 + 4 * lg + r) * PITCH + j * 16 + lr;
-        if (!__builtin_isfinite(*at)) *at = exact[r];
+        for (int x = 1; x < L; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+        bad_a |= uint32_t(lossy(ra.y, top)) << i;
       }
     }
-  }
+    bool bad_b[4], live_b = false, any_b = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+      for (int x = L; x < 64; x <<= 1) top_b[e] = fmaxf(top_b[e], __shfl_xor(top_b[e], x, 64));
+      bad_b[e] = lossy(rb[e].y, top_b[e]);
+      any_b = any_b || bad_b[e];
+      live_b = live_b || rb[e].x != kNothing;
+    }
+    live_a = __any(live_a);
+    live_b = __any(live_b);  // beside zeros nothing shows
+    if (__any(again || (bad_a && live_b) || (any_b && live_a))) {
+#pragma unroll 1
+      for (int i = 0; i < ROWS * L / 64; ++i) {
+        float* at = mine + (i * (64 / L) + y0) * PITCH + x4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((live_b && (bad_a >> i & 1)) || (live_a && bad_b[e])) at[e] = __builtin_inff();
+      }
+#pragma unroll 1
+      for (int f = 0; f < FM * FH; ++f) {
+        const int i = f / FH, j = f % FH;
+        f32x4 exact = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int k = s0 * 32 + lg; k < s1 * 32 + lg; k += 4)
+          exact = mfma_f32(element_a(a.s, a.product, mw + i * 16 + lr, k), element_b(a.s, a.product, nw + j * 16 + lr, k), exact);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float* at = mine + (i * 16 + 4 * lg + r) * PITCH + j * 16 + lr;
+          if (!__builtin_isfinite(*at)) *at = exact[r];
+        }
+      }
+    }
 
-  if (a.wide) put_tile<4, ROWS, COLS, PITCH>(a, split, mine, mw, nw, lane);
-  else put_tile<1, ROWS, COLS, PITCH>(a, split, mine, mw, nw, lane);
+    if (a.wide) put_tile<4, ROWS, COLS, PITCH>(a, split, mine, mw, nw, lane);
+    else put_tile<1, ROWS, COLS, PITCH>(a, split, mine, mw, nw, lane);
   }
 }
 
@@ -733,11 +748,13 @@ __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
   if (to) to[c < N ? c : c - N] = float(t);
 }
 
-// ------------------------------------------------------------- few rows ---
+// ------------------------------------------------------- small products ---
 
-// 16 columns of both projections and up to 16 RB rows: the weights go from
-// memory into the products' registers, the wavefronts share K and their sums
-// meet in LDS, in order.  XV: x in whole 16-byte rows.
+// 16 columns of both projections and 16 RB rows: the weights go from memory
+// into the products' registers, the wavefronts share K and their sums meet in
+// LDS, in order.  XV: x in whole 16-byte rows.  Bound: at one row the launch and
+// two memory round trips (512 x 2048, 8.4 MB of weights: 5.0 us, 1.7 TB/s), with
+// many the FP32 matrix rate.
 struct FewArgs {
   const float *x, *wg, *wu;
   MmaArgs out;
@@ -754,6 +771,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
   const uint32_t bytes = uint32_t(K) * uint32_t(N) * 4u;
   const __amdgpu_buffer_rsrc_t rg = make_res(a.wg, bytes), ru = make_res(a.wu, bytes);
   const int blocks = (K + 15) / 16, per = (blocks + kFewWaves - 1) / kFewWaves;
+  const int m0 = int(blockIdx.y) * 16 * RB;
   f32x4 acc[2][RB];
 #pragma unroll
   for (int q = 0; q < 2; ++q)
@@ -776,7 +794,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
       }
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        const int m = b * 16 + lr;
+        const int m = m0 + b * 16 + lr;
         if constexpr (XV) {
           x[d][b] = ld_f4(rx, in && m < M && k < K ? (uint32_t(m) * uint32_t(K) + uint32_t(k)) * 4u : ~0u - 15u);
         } else {
@@ -803,7 +821,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
       for (int r = 0; r < 4; ++r) part[wave][(q * RB + b) * 256 + (4 * lg + r) * 16 + lr] = acc[q][b][r];
   __syncthreads();
   for (int i = tid; i < RB * 256; i += 64 * kFewWaves) {
-    const int m = i >> 4, c = int(blockIdx.x) * 16 + (i & 15);
+    const int m = m0 + (i >> 4), c = int(blockIdx.x) * 16 + (i & 15);
     if (m >= M || c >= N) continue;
     float g = 0.f, u = 0.f;
 #pragma unroll
@@ -820,12 +838,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 long up_to(long n, long q) { return (n + q - 1) / q * q; }
 
-// Rows that read the weights as they are: beyond, packing them pays.
-constexpr int kFewRows = 32;
+// Products that read their operands as they are: beyond, packing pays.  Forward
+// alone, calls one after another, this way and packed, us: K 512, N 2048 with 128
+// rows 9.9 / 25, 256 18 / 26, 512 32 / 29; 1024, 4096 with 32 13 / 36, 64 19 / 37, 192
+// 49 / 40; 2048, 1024 with 256 29 / 35, 300 53 / 38; 777 x 500 x 1333 51 / 37.
+constexpr long kFewWork = 1L << 28;
+bool few_products(const ttrl_gated_desc* d) { return long(d->M) * d->K <= kFewWork / d->N; }
 
-// A product's tiles and splits: 256 x 128 where they fill the compute units
-// (or nearly), else 64 x 64, and k in splits while there are fewer workgroups
-// than two a compute unit and a split keeps kMinSteps steps.
+// A product's tiles and splits: 256 x 256 where they fill three quarters of the
+// compute units, counting what shares the launch, else 64 x 64, and k in splits
+// while there are fewer workgroups than two a compute unit and a split keeps
+// kMinSteps steps.  Both ways, us: 128 tiles of 256 x 256 at 2048 x 512 x 2048 205,
+// 64 x 64 158; at 8192 x 256 x 1024 259 and 227; at 8192 x 1024 x 4096 256 x 256 1429
+// and 256 x 128 1510.  128 x 64 took 94 at 777 x 500 x 1333, 64 x 64 92.
 constexpr int kMinSteps = 6;
 struct MmaPlan {
   bool big;
@@ -995,7 +1020,7 @@ int ttrl_gated_space(const ttrl_gated_desc* d, long* forward_bytes, long* backwa
   if (int rc = check_gated(d, "ttrl_gated_space")) return rc;
   TTRL_REQUIRE(forward_bytes && backward_bytes, "ttrl_gated_space: null output");
   const Layouts l = layouts_of(d);
-  *forward_bytes = d->M <= kFewRows ? 0 : l.fwd.a + l.fwd.b + l.fwd.rows + l.fwd_max + l.fwd.part;
+  *forward_bytes = few_products(d) ? 0 : l.fwd.a + l.fwd.b + l.fwd.rows + l.fwd_max + l.fwd.part;
   *backward_bytes = l.dx.a + l.dx.b + l.dx.rows + l.dw.a + l.dw.b + l.dw.rows + l.bwd_max +
                     l.dx.part + l.dw.part + l.sums;
   return TTRL_OK;
@@ -1016,17 +1041,19 @@ int ttrl_gated_forward(ttrl_ctx* ctx, const ttrl_gated_desc* d) {
   m.o1 = d->g;
   m.o2 = d->u;
   m.s = source_of(d);
-  if (d->M <= kFewRows) {
+  if (few_products(d)) {
     const FewArgs f{d->x, d->w_gate, d->w_up, m};
-    const dim3 grid(ceil_div(d->N, 16)), block(64 * kFewWaves);
+    const int rb = d->M <= 16 ? 1 : d->M <= 32 ? 2 : 4;
+    const dim3 grid(ceil_div(d->N, 16), ceil_div(d->M, 16 * rb)), block(64 * kFewWaves);
     const bool xv = d->K % 4 == 0 && aligned16(d->x);
     auto go = [&](auto rb) {
       constexpr int RB = decltype(rb)::value;
       if (xv) hipLaunchKernelGGL((k_few<RB, true>), grid, block, 0, stream_of(ctx), f);
       else hipLaunchKernelGGL((k_few<RB, false>), grid, block, 0, stream_of(ctx), f);
     };
-    if (d->M <= 16) go(std::integral_constant<int, 1>{});
-    else go(std::integral_constant<int, 2>{});
+    if (rb == 1) go(std::integral_constant<int, 1>{});
+    else if (rb == 2) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 4>{});
     return check_launch(name);
   }
   TTRL_REQUIRE(d->work && aligned16(d->work), "%s: null or unaligned workspace", name);
