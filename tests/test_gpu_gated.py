@@ -222,7 +222,7 @@ def test_small_values_beside_large_ones_that_meet_zeros(device, M):
 # Products large enough to be packed forward too, in small and large tiles;
 # ragged in every extent.
 @pytest.mark.parametrize("M,K,N,act,bias", [(2050, 523, 517, "gelu", True), (1031, 1029, 520, "relu", False),
-                                            (4100, 100, 1501, "sigmoid", True), (4100, 1500, 2100, "silu", False)])
+                                            (4100, 100, 1501, "sigmoid", True), (4100, 1500, 2100, "silu", False), (26000, 300, 260, "gelu", True)])
 def test_packed_products(device, M, K, N, act, bias):
     x, dh = _inputs(M, M, K, N, bias)
     if act == "relu":
@@ -263,3 +263,9 @@ def test_packed_products_of_small_values_beside_large_ones(device):
     x["x"] *= np.float32(2.0) ** np.linspace(-60, 12, 2050).astype(np.float32)[:, None]
     dh *= np.float32(2.0) ** np.linspace(20, -40, 2050).astype(np.float32)[:, None]
     _check(_run(device, x, "sigmoid", dh), x, "sigmoid", dh)
+
+
+def test_very_many_rows(device):
+    """More rows than a grid has workgroups in y (64 rows each)."""
+    x, dh = _inputs(13, 64 * 65535 + 70, 2, 3, True)
+    _check(_run(device, x, "silu", dh), x, "silu", dh)

@@ -43,7 +43,7 @@
 // packing writes 4 bytes a value beside the 4 read.  Where the time of that pass
 // goes (us): forward scan 13, pack 21, product 404; backward scan 120, pack 275
 // (1.1 GB, 4 TB/s), both products 604.
-#include "split_gemm.hpp"
+#include "tile_gemm.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -843,7 +843,9 @@ long up_to(long n, long q) { return (n + q - 1) / q * q; }
 // rows 9.9 / 25, 256 18 / 26, 512 32 / 29; 1024, 4096 with 32 13 / 36, 64 19 / 37, 192
 // 49 / 40; 2048, 1024 with 256 29 / 35, 300 53 / 38; 777 x 500 x 1333 51 / 37.
 constexpr long kFewWork = 1L << 28;
-bool few_products(const ttrl_gated_desc* d) { return long(d->M) * d->K <= kFewWork / d->N; }
+bool few_products(const ttrl_gated_desc* d) {
+  return long(d->M) * d->K <= kFewWork / d->N && d->M <= 64 * 65535;  // 64 rows to each of a grid's y
+}
 
 // A product's tiles and splits: 256 x 256 where they fill three quarters of the
 // compute units, counting what shares the launch, else 64 x 64, and k in splits
