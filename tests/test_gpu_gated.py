@@ -269,3 +269,44 @@ def test_very_many_rows(device):
     """More rows than a grid has workgroups in y (64 rows each)."""
     x, dh = _inputs(13, 64 * 65535 + 70, 2, 3, True)
     _check(_run(device, x, "silu", dh), x, "silu", dh)
+
+
+# One value of a row (the values that one output sums over) far above the rest,
+# that meets zeros in every second column of the other operand: half of the sums
+# have no part of it, beside others that have.
+@pytest.mark.parametrize("outlier", [1e6, 1e7, 1e9, 1e12])
+@pytest.mark.parametrize("product", ["forward", "input", "weight"])
+@pytest.mark.parametrize("M,K,N", [(300, 64, 48), (2050, 520, 516)])
+def test_large_values_that_meet_zeros_in_some_columns(device, M, K, N, product, outlier):
+    x, dh = _beside(21, M, K, N, product, outlier)
+    _check(_run(device, x, "sigmoid", dh), x, "sigmoid", dh)
+
+
+@pytest.mark.parametrize("product,M,K,N", [("forward", 16500, 130, 600), ("input", 4100, 1500, 2100), ("weight", 4100, 1500, 2100)])
+def test_large_values_that_meet_zeros_in_large_tiles(device, M, K, N, product):
+    x, dh = _beside(22, M, K, N, product, 1e9)
+    _check(_run(device, x, "sigmoid", dh), x, "sigmoid", dh)
+
+
+def _beside(seed, M, K, N, product, outlier):
+    x, dh = _inputs(seed, M, K, N, False)
+    if product == "forward":
+        x["x"][:, 5] = outlier
+        x["w_gate"][5, 1::2] = x["w_up"][5, 1::2] = 0
+    elif product == "input":
+        dh[:, 7] = outlier
+        x["w_gate"][1::2, 7] = x["w_up"][1::2, 7] = 0
+    else:
+        x["x"][11] *= np.float32(outlier)
+        dh[11, 1::2] = 0
+    return x, dh
+
+
+def test_sums_of_nothing_but_small_values(device):
+    """Inputs that are zero but for one step in a hundred, beside a gate whose
+    slopes reach down to 1e-9 of their largest: sums of few or no terms."""
+    x, dh = _inputs(23, 700, 90, 130, False)
+    rng = np.random.default_rng(24)
+    x["x"] *= rng.random(x["x"].shape) < 0.01
+    dh *= np.exp(-20 * rng.random(dh.shape)).astype(np.float32)
+    _check(_run(device, x, "silu", dh), x, "silu", dh)

@@ -27,8 +27,10 @@
 // three times per 32 k.  (Error against float64 at 8192 x 1024 x 4096: 1.1e-6 of
 // the largest, a library's FP32 products 1.7e-6.)  fp16 ends at 2^-24, so a
 // value under 2^-2 (2^-16 of its row's largest) is off by up to 2^-25 instead;
-// such values are counted by row, and where that count could show in a sum
-// (lossy() below), or a sum is not finite, it is formed again in FP32.
+// such values are counted by row, and every sum in which they could show (doubt()
+// and lossy_sums() below), or that is not finite, is formed again in FP32.  So a
+// sum is off by 2^-21 + 2^-22 of its terms' absolute values at most, beside FP32's
+// own rounding.
 //
 // (Three bf16 parts, 24 bits at any exponent, need six products and no scale:
 // the forward and backward pass of 8192 x 1024 x 4096 took 2651 us so, 1546
@@ -79,19 +81,13 @@ __device__ __forceinline__ f32x4 mfma_f32(float a, float b, const f32x4& c) {
 
 // ------------------------------------------------------------- operands ---
 
-// What a product's operands are made of, element by element (k_mma's second
-// way, and k_pack's sources).
+// What a product's operands are made of (k_pack's sources, and those of sums
+// that are formed again).
 struct Source {
   const float *x, *wg, *wu;      // (M, K), (K, N)
   const float *dh, *g, *u;       // (M, N)
   int M, K, N, act;
   int N32;                       // N in whole steps of 32
-  __device__ __forceinline__ float slope_of(long m, int n, int up) const {
-    const long at = m * N + n;
-    float s;
-    const float a = gate(act, g[at], &s);
-    return up ? dh[at] * a : dh[at] * u[at] * s;
-  }
 };
 enum Product { kForward, kInput, kWeight };
 // Columns of both projections lie in blocks of 16 in turn: 16 of gate, 16 of up.
@@ -99,34 +95,24 @@ __device__ __forceinline__ int column_of(int n, int* up) {
   *up = n >> 4 & 1;
   return (n >> 5) * 16 + (n & 15);
 }
-__device__ float element_a(const Source& s, int product, long m, int k) {
-  if (product == kForward) return m < s.M && k < s.K ? s.x[m * s.K + k] : 0.f;
-  if (product == kWeight) return m < s.K && k < s.M ? s.x[long(k) * s.K + m] : 0.f;
-  const int up = k >= s.N32, n = k - up * s.N32;
-  return m < s.M && n < s.N ? s.slope_of(m, n, up) : 0.f;
-}
-__device__ float element_b(const Source& s, int product, int n, int k) {
-  int up;
-  if (product == kInput) {
-    up = k >= s.N32;
-    const int c = k - up * s.N32;
-    return n < s.K && c < s.N ? (up ? s.wu : s.wg)[long(n) * s.N + c] : 0.f;
-  }
-  const int c = column_of(n, &up);
-  if (c >= s.N) return 0.f;
-  if (product == kForward) return k < s.K ? (up ? s.wu : s.wg)[long(k) * s.N + c] : 0.f;
-  return k < s.M ? s.slope_of(k, c, up) : 0.f;
-}
 
 constexpr int kParts = 2, kPart = 1024, kFrag = kParts * kPart;  // bytes of 16 x 32 values: a part, both
 
+// What is known of a packed row.
+struct __attribute__((aligned(16))) Row {
+  int scale;  // the exponent of the largest value less 14
+  int small;  // values that fp16 ends above: not zero and, scaled, under 2^-2
+  int solid;  // values that are 2^8 and more, scaled, in every `sample`-th step
+  int unused;
+};
 // A matrix packed by rows (k along its columns) and by columns (k along its
 // rows), either or both.  Block b of 16 rows, step s of 32 k is fragment
 // (b * mul + add) * steps + s + first.
 struct Packed {
   char* p;
   int steps, first, mul, add;
-  int2* rows;  // of packed row r: the exponent of its largest value less 14; how many values fp16 ends above
+  Row* rows;
+  int sample;  // a power of two
 };
 struct PackJob {
   const float* src;  // plain matrix (R, C), or null: both slopes of the Source
@@ -262,28 +248,40 @@ __global__ __launch_bounds__(256) void k_scales(ScaleArgs a) {
   m = max(max(m, top[tid + 64]), max(top[tid + 128], top[tid + 192]));
   const int at = ((r >> 4) * j.to.mul + j.to.add) * 16 + (r & 15);
   const int e = m >> 23 ? int(m >> 23) - 127 : 31 - __clz(int(m)) - 149;
-  j.to.rows[at] = make_int2(m ? e - 14 : kNothing, 0);
+  j.to.rows[at] = Row{m ? e - 14 : kNothing, 0, 0, 0};
 }
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+// h of a value that is not zero and too small for fp16; zeros are 0.
+#define kTiny (-_Float16(0))
+
 // A lane's 8 values of a fragment, scaled and split.
 __device__ __forceinline__ void put_fragment(const Packed& to, int block, int step, int lane, int scale, const float (&v)[8]) {
   f16x8 h, l;
-  int small = 0;
+  int small = 0, solid = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float x = scale == kNothing ? 0.f : __builtin_ldexpf(v[i], -scale);
     h[i] = _Float16(x);
     l[i] = _Float16(x - float(h[i]));
+    if (h[i] == _Float16(0)) h[i] = x == 0.f ? _Float16(0) : kTiny;
     small += fabsf(x) < 0.25f && v[i] != 0.f;
+    solid += fabsf(x) >= 256.f;
   }
   char* at = to.p + (long(block * to.mul + to.add) * to.steps + step + to.first) * kFrag + lane * 16;
   *reinterpret_cast<f16x8*>(at) = h;
   *reinterpret_cast<f16x8*>(at + kPart) = l;
-  small += __shfl_xor(small, 16, 64);
-  small += __shfl_xor(small, 32, 64);
-  if (small && lane < 16) atomicAdd(&to.rows[(block * to.mul + to.add) * 16 + lane].y, small);  // a count: any order gives the same
+  const bool sampled = ((step + to.first) & (to.sample - 1)) == 0;  // uniform
+  if (!sampled && !__any(small)) return;
+  int both = small << 16 | solid;
+  both += __shfl_xor(both, 16, 64);
+  both += __shfl_xor(both, 32, 64);
+  if (lane < 16) {  // counts: any order gives the same
+    Row* row = to.rows + (block * to.mul + to.add) * 16 + lane;
+    if (sampled && (both & 0xffff)) atomicAdd(&row->solid, both & 0xffff);
+    if (both >> 16) atomicAdd(&row->small, both >> 16);
+  }
 }
 
 // A workgroup takes 32 x 64 values through LDS and writes them in both orders.
@@ -304,8 +302,8 @@ __device__ __forceinline__ void pack_tile(const PackJob& j, const Source& s, int
 #pragma unroll
   for (int p = 0; p < PARTS; ++p) {
     const Packed &r = j.rows[p], &k = j.cols[p];
-    if (r.p && in_r) scale_r[p] = r.rows[(rb * r.mul + r.add) * 16 + lr].x;
-    if (k.p && in_c) scale_c[p] = k.rows[(cb * k.mul + k.add) * 16 + lr].x;
+    if (r.p && in_r) scale_r[p] = r.rows[(rb * r.mul + r.add) * 16 + lr].scale;
+    if (k.p && in_c) scale_c[p] = k.rows[(cb * k.mul + k.add) * 16 + lr].scale;
   }
   float v[SLOPES ? 3 : 1][EACH];  // a thread's values, 4 rows apart, in flight together
 #pragma unroll
@@ -378,8 +376,9 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
 
 struct MmaArgs {
   const char *a, *b;  // packed operands
-  const int2 *rows_a, *rows_b;  // see Packed
+  const Row *rows_a, *rows_b;
   int product;
+  int places;                // of the sampled steps
   int M, N;                  // rows of a and of b
   int steps, per;            // steps of 32 k, of a split
   int tiles_m, tiles_n, splits;
@@ -506,9 +505,117 @@ __device__ __forceinline__ f32x4 mfma_f16(f16x8 a, f16x8 b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Whether `small` values, each off by up to 2^-25 and multiplied by up to 2^15,
-// could show beside the largest sum of their row (or column) at 2^-22.
-__device__ __forceinline__ bool lossy(int small, float top) { return small && top < 4096.f * float(small); }
+// Whether values that fp16 ends above could show in a sum at 2^-22 of its terms'
+// absolute values, or it is not finite.  Each of them is off by up to 2^-25 and
+// multiplied by up to 2^15, 2^-10 together; the terms amount to |sum| at least, and
+// to 2^16 for every place where row and column are both solid: among the sampled
+// places as many as both have solid ones beyond the number of places.  The
+// second holds nearly everywhere in dense operands; the first decides where
+// zeros meet large values.  It is asked of every sum, since the sums of other
+// columns say nothing about it.  (Counting in every step kept packing 100 us
+// longer at 8192 x 1024 x 4096.)
+struct Guard {
+  float spare, least;  // of a row's and a column's: solid places beyond what the small ones need; the sum that hides them
+  __device__ __forceinline__ Guard(const Row& r, int places)
+      : spare(float(r.solid - places) * 16.f - float(r.small)), least(float(r.small) * 4096.f) {}
+};
+__device__ __forceinline__ bool doubt(const Guard& a, const Guard& b, float sum) {
+  const float size = fabsf(sum);
+  return !((a.spare + b.spare >= 0.f || size >= a.least + b.least) && size < __builtin_inff());
+}
+
+// Magnitudes of a fragment's values, and 1 where fp16 ends above them.
+__device__ __forceinline__ void magnitudes(f16x8 h, f16x8* size, f16x8* small) {
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  const u16x8 v = __builtin_bit_cast(u16x8, h);
+  u16x8 m, one;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    m[i] = v[i] == 0x8000 ? 1 : v[i] & 0x7fff;  // kTiny: the least there is
+    one[i] = v[i] && m[i] < 0x3400 ? 0x3c00 : 0;
+  }
+  *size = __builtin_bit_cast(f16x8, m);
+  *small = __builtin_bit_cast(f16x8, one);
+}
+
+// Where counts leave a doubt about 16 rows, pairs decide: the terms' absolute
+// values and, in units of 2^-25, what the small values among them may be off by
+// are formed from the h parts.  Sums in which that could show become infinite
+// in the wavefront's results.  The factor leaves h's rounding to what the counts
+// have passed.
+template <int FH, int PITCH>
+__device__ __forceinline__ void lossy_sums(const char* a, const char* b, long pitch, int s0, int s1, float* at) {
+  f32x4 terms[FH], off[FH];
+#pragma unroll
+  for (int j = 0; j < FH; ++j) terms[j] = off[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int s = s0; s < s1; ++s) {
+    f16x8 ha, hb[FH], size_a, small_a;
+    ha = *reinterpret_cast<const f16x8*>(a + long(s) * kFrag);
+#pragma unroll
+    for (int j = 0; j < FH; ++j) hb[j] = *reinterpret_cast<const f16x8*>(b + j * pitch + long(s) * kFrag);
+    magnitudes(ha, &size_a, &small_a);
+#pragma unroll
+    for (int j = 0; j < FH; ++j) {
+      f16x8 size_b, small_b;
+      magnitudes(hb[j], &size_b, &small_b);
+      terms[j] = mfma_f16(size_a, size_b, terms[j]);
+      off[j] = mfma_f16(small_a, size_b, off[j]);
+      off[j] = mfma_f16(size_a, small_b, off[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < FH; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (!(off[j][r] <= 8.03125f * terms[j][r])) at[r * PITCH + j * 16] = __builtin_inff();
+}
+
+// A fragment's sums in FP32 from the plain operands, steps s0 to s1.  Addresses
+// past the ends stay on the last element, so that nothing branches and a step's
+// loads are in flight together.
+template <int PRODUCT>
+__device__ __forceinline__ f32x4 plain_sums(const Source& s, long m, int n, int s0, int s1, int lg) {
+  f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+  int up = 0;
+  const int c = PRODUCT == kInput ? n : column_of(n, &up);  // its column (of dx: weight row)
+  const bool in_n = c < (PRODUCT == kInput ? s.K : s.N), in_m = m < (PRODUCT == kWeight ? s.K : s.M);
+  const long mc = min(m, long(PRODUCT == kWeight ? s.K : s.M) - 1);
+  const int nc = min(c, (PRODUCT == kInput ? s.K : s.N) - 1);
+#pragma unroll 1
+  for (int step = s0; step < s1; ++step) {
+    float a[8], b[8], d[PRODUCT == kForward ? 1 : 3][8];
+    const bool second = PRODUCT == kInput && step * 32 >= s.N32;  // of both projections' columns
+    const bool of_up = PRODUCT == kInput ? second : up != 0;
+    const float* w = of_up ? s.wu : s.wg;
+    const int k0 = step * 32 - (second ? s.N32 : 0) + lg, K = PRODUCT == kForward ? s.K : PRODUCT == kInput ? s.N : s.M;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const long k = min(k0 + 4 * q, K - 1), at = PRODUCT == kInput ? mc * s.N + k : k * s.N + nc;
+      if constexpr (PRODUCT == kForward) {
+        a[q] = s.x[mc * s.K + k];
+        b[q] = w[at];
+      } else {
+        if constexpr (PRODUCT == kInput) b[q] = w[long(nc) * s.N + k];
+        else a[q] = s.x[k * s.K + mc];
+        d[0][q] = s.g[at];
+        d[1][q] = s.u[at];
+        d[2][q] = s.dh[at];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if constexpr (PRODUCT != kForward) {
+        float slope;
+        const float act = gate(s.act, d[0][q], &slope);
+        (PRODUCT == kInput ? a[q] : b[q]) = of_up ? d[2][q] * act : d[2][q] * d[1][q] * slope;
+      }
+      const bool in_k = k0 + 4 * q < K;
+      sum = mfma_f32(in_m && in_k ? a[q] : 0.f, in_n && in_k ? b[q] : 0.f, sum);
+    }
+  }
+  return sum;
+}
 
 // WM x WN wavefronts of FM x FN fragments of 16 x 16, BUFS steps of operands in
 // LDS.  256 x 256 tiles run at 1.02 (forward, with the activation and three
@@ -613,75 +720,58 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) mine[(i * 16 + 4 * lg + r) * PITCH + j * 16 + lr] = acc[i][x * FH + j][r];
 
-    // Scales taken out.  Sums that are not finite, and rows and columns whose
-    // small values could show, are formed again in FP32, each by its own row or
-    // column, measured by its largest sum among the wavefront's.
+    // Scales taken out, sums in doubt looked into and formed again.
     const int x4 = lane % L * 4, y0 = lane / L;
-    int2 rb[4];
-    float top_b[4] = {};
+    int scale_b[4];
+    Guard guard_b[4] = {{Row{}, 0}, {Row{}, 0}, {Row{}, 0}, {Row{}, 0}};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      rb[e] = make_int2(kNothing, 0);
-      if (nw + x4 + e < a.N) rb[e] = a.rows_b[nw + x4 + e];
+      scale_b[e] = kNothing;
+      if (nw + x4 + e < a.N) {
+        const Row r = a.rows_b[nw + x4 + e];
+        scale_b[e] = r.scale;
+        guard_b[e] = Guard(r, a.places);
+      }
     }
-    bool again = false, live_a = false;
-    uint32_t bad_a = 0;  // bit i: this lane's i-th row
+    uint32_t again = 0;  // bit i: in 16 rows
 #pragma unroll 2
     for (int i = 0; i < ROWS * L / 64; ++i) {
       const int y = i * (64 / L) + y0;
-      int2 ra = make_int2(kNothing, 0);
+      Row ra{kNothing, 0, 0, 0};
       if (mw + y < a.M) ra = a.rows_a[mw + y];
+      const Guard guard_a(ra, 0);
       f32x4* at = reinterpret_cast<f32x4*>(mine + y * PITCH + x4);
       f32x4 v = *at;
-      float top = 0.f;
+      bool bad = false;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (ra.x == kNothing || rb[e].x == kNothing) v[e] = 0.f;  // and rows nobody packed
-        const bool fin = __builtin_isfinite(v[e]);
-        again = again || !fin;
-        const float size = fin ? fabsf(v[e]) : 0.f;
-        top = fmaxf(top, size);
-        top_b[e] = fmaxf(top_b[e], size);
-        v[e] = __builtin_ldexpf(v[e], ra.x + rb[e].x);
+        const bool none = ra.scale == kNothing || scale_b[e] == kNothing;  // zeros, and rows nobody packed
+        bad = bad || (!none && doubt(guard_a, guard_b[e], v[e]));
+        v[e] = none ? 0.f : __builtin_ldexpf(v[e], ra.scale + scale_b[e]);
       }
       *at = v;
-      live_a = live_a || ra.x != kNothing;
-      if (__any(ra.y)) {
-#pragma unroll
-        for (int x = 1; x < L; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-        bad_a |= uint32_t(lossy(ra.y, top)) << i;
-      }
+      again |= uint32_t(bad) << (i * (64 / L) / 16);
     }
-    bool bad_b[4], live_b = false, any_b = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-      for (int x = L; x < 64; x <<= 1) top_b[e] = fmaxf(top_b[e], __shfl_xor(top_b[e], x, 64));
-      bad_b[e] = lossy(rb[e].y, top_b[e]);
-      any_b = any_b || bad_b[e];
-      live_b = live_b || rb[e].x != kNothing;
-    }
-    live_a = __any(live_a);
-    live_b = __any(live_b);  // beside zeros nothing shows
-    if (__any(again || (bad_a && live_b) || (any_b && live_a))) {
+    if (__any(again)) {
 #pragma unroll 1
-      for (int i = 0; i < ROWS * L / 64; ++i) {
-        float* at = mine + (i * (64 / L) + y0) * PITCH + x4;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((live_b && (bad_a >> i & 1)) || (live_a && bad_b[e])) at[e] = __builtin_inff();
-      }
+      for (int i = 0; i < FM; ++i) {
+        const long m = mw + i * 16;
+        if (!__any(again >> i & 1) || m >= a.M) continue;
+        float* at = mine + (i * 16 + 4 * lg) * PITCH + lr;
+        lossy_sums<FH, PITCH>(a.a + (m / 16) * pitch + lane * 16, a.b + long(nw / 16) * pitch + lane * 16, pitch, s0, s1, at);
 #pragma unroll 1
-      for (int f = 0; f < FM * FH; ++f) {
-        const int i = f / FH, j = f % FH;
-        f32x4 exact = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-        for (int k = s0 * 32 + lg; k < s1 * 32 + lg; k += 4)
-          exact = mfma_f32(element_a(a.s, a.product, mw + i * 16 + lr, k), element_b(a.s, a.product, nw + j * 16 + lr, k), exact);
+        for (int j = 0; j < FH; ++j, at += 16) {
+          const int n = nw + j * 16;
+          bool bad = false;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float* at = mine + (i * 16 + 4 * lg + r) * PITCH + j * 16 + lr;
-          if (!__builtin_isfinite(*at)) *at = exact[r];
+          for (int r = 0; r < 4; ++r) bad = bad || !__builtin_isfinite(at[r * PITCH]);
+          if (!__any(bad) || n >= a.N) continue;
+          const f32x4 exact = a.product == kForward ? plain_sums<kForward>(a.s, m + lr, n + lr, s0, s1, lg)
+                              : a.product == kInput ? plain_sums<kInput>(a.s, m + lr, n + lr, s0, s1, lg)
+                                                    : plain_sums<kWeight>(a.s, m + lr, n + lr, s0, s1, lg);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!__builtin_isfinite(at[r * PITCH])) at[r * PITCH] = exact[r];
         }
       }
     }
@@ -878,17 +968,22 @@ struct Layout {
   long a, b, rows, part;  // bytes
   MmaPlan plan;
   long rows_a, rows_b;
-  int steps;
+  int steps, sample, places;
 };
-Layout layout_of(long M, long N, long steps, int together) {
+constexpr int kSampled = 8;  // steps whose solid values are counted, at most
+// `terms` of a sum lie in whole steps of 32, twice over where there are two `halves`.
+Layout layout_of(long M, long N, long terms, int halves, int together) {
   Layout l{};
-  l.plan = plan_mma(M, N, steps, together);
+  const long steps = (terms + 31) / 32;
+  l.steps = int(steps * halves);
+  for (l.sample = 1; l.sample * kSampled < l.steps;) l.sample *= 2;
+  for (long s = 0; s < l.steps; s += l.sample) l.places += int(std::min(32L, terms - s % steps * 32));
+  l.plan = plan_mma(M, N, l.steps, together);
   l.rows_a = M;
   l.rows_b = N;
-  l.steps = int(steps);
-  l.a = up_to(M, 256) / 16 * steps * kFrag;  // whole tiles are read, whatever lies there
-  l.b = up_to(N, 256) / 16 * steps * kFrag;
-  l.rows = up_to((up_to(M, 16) + up_to(N, 16)) * 8, 256);
+  l.a = up_to(M, 256) / 16 * l.steps * kFrag;  // whole tiles are read, whatever lies there
+  l.b = up_to(N, 256) / 16 * l.steps * kFrag;
+  l.rows = up_to((up_to(M, 16) + up_to(N, 16)) * long(sizeof(Row)), 256);
   l.part = l.plan.splits > 1 ? up_to(long(l.plan.splits) * M * N * 4, 256) : 0;
   return l;
 }
@@ -897,8 +992,8 @@ struct Operands {
   Packed a, b;
 };
 Operands operands_at(const Layout& l, char* at) {
-  int2* rows = reinterpret_cast<int2*>(at + l.a + l.b);
-  return Operands{Packed{at, l.steps, 0, 1, 0, rows}, Packed{at + l.a, l.steps, 0, 1, 0, rows + up_to(l.rows_a, 16)}};
+  Row* rows = reinterpret_cast<Row*>(at + l.a + l.b);
+  return Operands{Packed{at, l.steps, 0, 1, 0, rows, l.sample}, Packed{at + l.a, l.steps, 0, 1, 0, rows + up_to(l.rows_a, 16), l.sample}};
 }
 Packed moved(Packed p, int first, int mul, int add) {
   p.first = first;
@@ -914,11 +1009,11 @@ struct Layouts {
   long fwd_max, bwd_max, sums;  // bytes of the scans' results and of the column sums
 };
 Layouts layouts_of(const ttrl_gated_desc* d) {
-  const long rows = std::max(1, d->M), both = up_to(d->N, 16) * 2, n32 = (d->N + 31) / 32;
+  const long rows = std::max(1, d->M), both = up_to(d->N, 16) * 2;
   Layouts l;
-  l.fwd = layout_of(rows, both, (d->K + 31) / 32, 1);
-  l.dx = layout_of(rows, d->K, 2 * n32, 2);
-  l.dw = layout_of(d->K, both, (rows + 31) / 32, 2);
+  l.fwd = layout_of(rows, both, d->K, 1, 1);
+  l.dx = layout_of(rows, d->K, d->N, 2, 2);
+  l.dw = layout_of(d->K, both, rows, 1, 2);
   l.fwd_max = up_to((scan_cols(d->K) * rows + 2 * scan_rows(d->K) * d->N) * 4, 256);
   l.bwd_max = up_to((scan_cols(d->N) * (rows + 2L * d->K) + scan_rows(rows) * (2L * d->N + d->K)) * 4, 256);
   l.sums = up_to((rows + 31) / 32 * 2 * d->N * 4, 256);
@@ -970,6 +1065,7 @@ void fill_in(MmaArgs& a, const Layout& l, const Operands& o, float* part) {
   a.M = int(l.rows_a);
   a.N = int(l.rows_b);
   a.steps = l.steps;
+  a.places = l.places;
   a.per = l.plan.per;
   a.tiles_m = l.plan.tiles_m;
   a.tiles_n = l.plan.tiles_n;
