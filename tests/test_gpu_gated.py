@@ -310,3 +310,37 @@ def test_sums_of_nothing_but_small_values(device):
     x["x"] *= rng.random(x["x"].shape) < 0.01
     dh *= np.exp(-20 * rng.random(dh.shape)).astype(np.float32)
     _check(_run(device, x, "silu", dh), x, "silu", dh)
+
+
+@pytest.mark.parametrize("M,K,N", [(3, 32, 64), (300, 32, 64), (2050, 520, 516)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_what_is_not_finite_shows_beside_zeros(device, M, K, N, bad):
+    """A product of zero and NaN or infinity is NaN, whether all of a row or
+    column is zero or not, in each product and at every size."""
+    def clean():
+        return _inputs(31, M, K, N, bias=False)
+
+    x, dh = clean()
+    x["w_gate"][:] = x["w_up"][:] = 0
+    x["x"][2, 5] = bad
+    out = _run(device, x, "silu", dh)["out"]
+    assert np.isnan(out[2]).all() and not np.delete(out, 2, 0).any()
+
+    x, dh = clean()
+    x["w_gate"][:, 9] = x["w_up"][:, 9] = 0
+    x["x"][2, 5] = bad
+    out = _run(device, x, "sigmoid", dh)["out"]
+    assert np.isnan(out[2, 9]) and np.isfinite(np.delete(out, 2, 0)).all()
+
+    x, dh = clean()  # dx: a weight row of zeros beside a slope that is not finite
+    x["w_gate"][4] = x["w_up"][4] = 0
+    dh[1, 3] = bad
+    dx = _run(device, x, "sigmoid", dh)["x"]
+    assert np.isnan(dx[1, 4]) and np.isfinite(np.delete(dx, 1, 0)).all()
+
+    x, dh = clean()  # dW: a feature of zeros beside it
+    x["x"][:, 4] = 0
+    dh[1, 3] = bad
+    got = _run(device, x, "sigmoid", dh)
+    for n in ("w_gate", "w_up"):
+        assert np.isnan(got[n][4, 3]) and np.isfinite(np.delete(got[n], 3, 1)).all(), n

@@ -229,7 +229,8 @@ struct ScaleArgs {
   ScaleJob job[kScales];
   int jobs;
 };
-constexpr int kNothing = -100000;  // the scale of a row of zeros
+constexpr int kNothing = -100000;      // the scale of a row of zeros
+constexpr int kUnbounded = 128 - 14;  // and of one that is not finite
 __global__ __launch_bounds__(256) void k_scales(ScaleArgs a) {
   __shared__ uint32_t top[256];
   int q = 0;
@@ -746,7 +747,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool none = ra.scale == kNothing || scale_b[e] == kNothing;  // zeros, and rows nobody packed
-        bad = bad || (!none && doubt(guard_a, guard_b[e], v[e]));
+        bad = bad || (none ? ra.scale == kUnbounded || scale_b[e] == kUnbounded : doubt(guard_a, guard_b[e], v[e]));
         v[e] = none ? 0.f : __builtin_ldexpf(v[e], ra.scale + scale_b[e]);
       }
       *at = v;
