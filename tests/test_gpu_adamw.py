@@ -215,3 +215,35 @@ def test_refusals(device):
     state["m"] = [a.astype(np.float32) for a in state["m"]]
     with pytest.raises(ValueError):
         opt.load_state_dict(state)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_what_is_not_finite_stays_in_the_moments(device, bad):
+    """In 8 bits a gradient that is not finite spoils both moments of its block
+    and no others', and they stay spoilt."""
+    from ttrl_amd.engine.optim import AdamW
+
+    shapes, at = [(200,), (10,)], 100
+    ends = []
+    for value in (0.0, bad):
+        params = _tensors(device, shapes, 7)
+        opt = AdamW(params, lr=LR, state_bits=8)
+        held = []
+        for s in range(3):
+            grads = _grads(np.random.default_rng(8 + s), shapes)
+            if s == 1:
+                grads[0][at] = value
+            _set_grads(device, params, grads)
+            opt.step()
+            held.append([[a.numpy() for a in side] for side in opt.moments()])
+        ends.append((held, opt.state_dict()))
+    (clean, _), (got, state) = ends
+    block = np.zeros(200, bool)
+    block[64:128] = True
+    for s in range(3):
+        for side in range(2):
+            a, b = got[s][side], clean[s][side]
+            assert np.array_equal(a[1], b[1]) and np.array_equal(a[0][~block], b[0][~block])
+            assert s == 0 or not np.isfinite(a[0][block]).any(), (s, side)
+    for name in ("m_scale", "v_scale"):
+        assert not np.isfinite(state[name][0][1]) and np.isfinite(state[name][0][[0, 2, 3]]).all()

@@ -109,10 +109,12 @@ __device__ __forceinline__ void store4(float* p, long i, long n, bool whole, con
     if (i + j < n) p[i + j] = x[j];
 }
 
+// A magnitude as bits, which order as magnitudes do, infinity and NaN above all.
+__device__ __forceinline__ uint32_t size_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
 // The largest over the 16 lanes (a DPP row) that hold a block.
-__device__ __forceinline__ float row_max(float x) {
-#define TTRL_ROW_ROR(n) \
-  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + n, 0xf, 0xf, true)))
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+#define TTRL_ROW_ROR(n) x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x120 + n, 0xf, 0xf, true)))
   TTRL_ROW_ROR(8);
   TTRL_ROW_ROR(4);
   TTRL_ROW_ROR(2);
@@ -135,21 +137,20 @@ __device__ __forceinline__ float held_v(unsigned code, float scale) {
 __device__ __forceinline__ int code_m(float m, float scale) {
 #pragma clang fp contract(off)
   const float r = scale > 0.f ? fabsf(m) / scale : 0.f;
-  const int c = int(rintf(sqrtf(r) * 127.f));
+  const int c = r > 0.f ? int(rintf(sqrtf(r) * 127.f)) : 0;  // 0 for NaN, whose block's scale tells
   return m < 0.f ? -c : c;
 }
 __device__ __forceinline__ unsigned code_v(float v, float scale) {
 #pragma clang fp contract(off)
   const float r = scale > 0.f ? v / scale : 0.f;
-  const float c = rintf(sqrtf(sqrtf(r)) * 255.f);
-  return unsigned(r > 0.f ? fmaxf(c, 1.f) : c);
+  return r > 0.f ? unsigned(fmaxf(rintf(sqrtf(sqrtf(r)) * 255.f), 1.f)) : 0u;
 }
 
 // Four elements' codes.  Divided and rooted by the hardware's approximations (1
 // ulp each), x = 127 sqrt(r) is off by under 4e-5 and 255 r^(1/4) by under 8e-5
 // where scale and r are far from the range's ends, and the correctly rounded
 // forms above by as much: no half step within kSure means the same code.  The
-// rest (one wavefront's round in ten or so) takes the forms above.  They cost
+// rest (one wavefront's round in five or so) takes the forms above.  They cost
 // two divisions and three roots an element, more time than the memory: 67M
 // parameters 327 us, 245 so, and 210 to 280 with the tickets' desks below.
 constexpr float kSure = 2e-4f;
@@ -164,9 +165,9 @@ __device__ __forceinline__ void codes4(const f32x4& m, const f32x4& v, float top
     const float y = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(r)) * 255.f;
     sure = sure && fabsf(__builtin_amdgcn_fractf(x) - 0.5f) > kSure && fabsf(__builtin_amdgcn_fractf(y) - 0.5f) > kSure &&
            (r > 1e-30f || v[j] == 0.f);
-    const int c = int(rintf(x));
+    const int c = int(fminf(rintf(x), 127.f));  // NaN, which is not sure, converts too
     a |= (uint32_t(m[j] < 0.f ? -c : c) & 255u) << (8 * j);
-    b |= uint32_t(v[j] > 0.f ? fmaxf(rintf(y), 1.f) : 0.f) << (8 * j);
+    b |= uint32_t(v[j] > 0.f ? fminf(fmaxf(rintf(y), 1.f), 255.f) : 0.f) << (8 * j);
   }
   if (!sure) {
     a = b = 0;
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw(AdamWArgs a) {
 #pragma unroll
   for (int u = 0; u < ROUNDS; ++u) {
     const long i = from + u * kRound, s = it.at + i;
-    float top_m = 0.f, top_v = 0.f;
+    uint32_t size_m = 0, size_v = 0;
     if (in[u]) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -242,8 +243,8 @@ __global__ __launch_bounds__(kThreads) void k_adamw(AdamWArgs a) {
         if (HELD && i + j >= n) mj = vj = 0.f;
         m[u][j] = mj;
         v[u][j] = vj;
-        top_m = fmaxf(top_m, fabsf(mj));
-        top_v = fmaxf(top_v, vj);
+        size_m = max(size_m, size_bits(mj));
+        size_v = max(size_v, size_bits(vj));
       }
       store4(it.p, i, n, whole[u], p[u]);
       if constexpr (!HELD) {
@@ -252,8 +253,7 @@ __global__ __launch_bounds__(kThreads) void k_adamw(AdamWArgs a) {
       }
     }
     if constexpr (HELD) {  // every lane of a row takes part
-      top_m = row_max(top_m);
-      top_v = row_max(top_v);
+      const float top_m = __uint_as_float(row_max(size_m)), top_v = __uint_as_float(row_max(size_v));
       if (in[u]) {
         uint32_t cm, cv;
         codes4(m[u], v[u], top_m, top_v, &cm, &cv);
