@@ -247,3 +247,57 @@ def test_what_is_not_finite_stays_in_the_moments(device, bad):
             assert s == 0 or not np.isfinite(a[0][block]).any(), (s, side)
     for name in ("m_scale", "v_scale"):
         assert not np.isfinite(state[name][0][1]) and np.isfinite(state[name][0][[0, 2, 3]]).all()
+
+
+# A set large enough that a workgroup takes four rounds, beside odd tensors off
+# 16 bytes; and one of 69 workgroups, which share the desks where they take tickets.
+LARGE = [(2053, 2049), (3, 1001), (77,), (1, 4096)]
+SHARED = [(200, 301), (9, 1000), (5,)]
+
+
+@pytest.mark.parametrize("shapes,offset,steps", [(LARGE, 0, 2), (LARGE, 1, 2), (SHARED, 0, 6), (SHARED, 1, 6)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_large_sets_match_the_host_bit_for_bit(device, shapes, offset, steps, bits):
+    from ttrl_amd.engine.optim import AdamW
+
+    params = _tensors(device, shapes, 13, offset)
+    opt = AdamW(params, lr=LR, betas=BETAS, eps=EPS, weight_decay=WD, state_bits=bits)
+    host = [(p.numpy().reshape(-1), np.zeros(p.data.numel, np.float32), np.zeros(p.data.numel, np.float32)) for p in params]
+    rng = np.random.default_rng(14)
+    for t in range(1, steps + 1):
+        grads = _grads(rng, shapes)
+        _set_grads(device, params, grads)
+        opt.step()
+        host = [_host_step(p, g.reshape(-1), m, v, t) for (p, m, v), g in zip(host, grads)]
+        if bits == 8:
+            host = [(p, O.held_m(*O.hold_m(m)), O.held_v(*O.hold_v(v))) for p, m, v in host]
+    m, v = opt.moments()
+    for i, (p, hm, hv) in enumerate(host):
+        for name, a, b in (("p", params[i], p), ("m", m[i], hm), ("v", v[i], hv)):
+            assert np.array_equal(a.numpy().reshape(-1), b), (i, name)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_of_many_workgroups_counts_by_itself(device, bits):
+    from ttrl_amd.engine.autograd import Tensor
+    from ttrl_amd.engine.ops import mean_all, square, sub
+    from ttrl_amd.engine.optim import AdamW
+    from ttrl_amd.engine.step import TrainStep
+
+    ends = []
+    for mode in ("eager", "graph"):
+        params = _tensors(device, [(200, 301), (1, 301), (200, 1)], 15)
+        opt = AdamW(params, lr=LR, betas=BETAS, state_bits=bits)
+        x = {"y": Tensor.from_numpy(np.ones((200, 301), np.float32), device)}
+
+        def body(x):
+            loss = mean_all(square(sub(params[0] + params[1] + params[2], x["y"])))
+            loss.backward()
+            return {}
+
+        with TrainStep(body, x, device, optimizer=opt, mode=mode) as step:
+            for _ in range(7):
+                step.run()
+            assert opt.t == 7
+            ends.append([p.numpy() for p in params])
+    assert all(np.array_equal(a, b) for a, b in zip(*ends))
