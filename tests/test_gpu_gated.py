@@ -344,3 +344,16 @@ def test_what_is_not_finite_shows_beside_zeros(device, M, K, N, bad):
     got = _run(device, x, "sigmoid", dh)
     for n in ("w_gate", "w_up"):
         assert np.isnan(got[n][4, 3]) and np.isfinite(np.delete(got[n], 3, 1)).all(), n
+
+
+# Forward products whose sums are formed in several parts: few tiles, a long sum.
+@pytest.mark.parametrize("M,K,N,act,bias", [(300, 1024, 1024, "silu", True), (100, 2100, 1333, "gelu", True),
+                                            (70, 4099, 1021, "sigmoid", False)])
+def test_packed_products_in_parts(device, M, K, N, act, bias):
+    x, dh = _inputs(41, M, K, N, bias)
+    _check(_run(device, x, act, dh), x, act, dh)
+
+
+def test_packed_products_in_parts_at_any_alignment(device):
+    x, dh = _inputs(42, 300, 1024, 1024, True)
+    _check(_run(device, x, "silu", dh, 1), x, "silu", dh)
