@@ -274,3 +274,37 @@ def test_refusals(device):
         linear_attention_step(t(2, 4, 8), t(2, 2, 8), t(2, 2, 6), g, None)
     with pytest.raises(RuntimeError):
         linear_attention_step(t(2, 4, 8, grad=True), t(2, 2, 8), t(2, 2, 6), g, s)
+
+
+# T, B, H, G, K, V, steps, resets, state, dfinal.  Sweeps that run through several
+# chunks and leave the states at every 256th step (256 heads and more), and ones
+# cut into segments of three to eight chunks, with widths of unlike tiles.
+LONG = [
+    (300, 32, 8, 4, 8, 12, True, 0.01, True, True),
+    (600, 64, 4, 4, 16, 8, False, 0.005, True, True),
+    (513, 86, 3, 1, 5, 33, True, None, True, False),
+    (767, 128, 2, 2, 4, 4, True, 0.003, False, True),
+    (700, 25, 4, 2, 16, 24, True, 0.01, True, True),
+    (1500, 2, 6, 3, 40, 72, True, 0.003, True, True),
+    (1500, 2, 6, 3, 40, 72, False, None, True, False),
+    (1111, 7, 3, 1, 33, 9, False, 0.002, False, True),
+]
+
+
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "-".join(str(x) for x in c))
+def test_many_chunks_match_the_oracle(device, case):
+    T, B, H, G, K, V = case[:6]
+    x, dout, dfinal = _inputs(T + B, *case)
+    if x["done"] is not None:  # resets at the ends of segments and beside them
+        for i, t in enumerate((95, 96, 97, 255, 256, 257, 511, 512, 513)):
+            if t < T:
+                x["done"][t, i % B] = 1
+    got = _run(device, x, dout, dfinal)
+    _check(got, *_wanted(x, dout, dfinal), K + V + T / 8 + 256)
+
+
+def test_many_chunks_at_any_alignment(device):
+    for case in ((300, 32, 8, 4, 8, 12, True, 0.01, True, True), (700, 25, 4, 2, 16, 24, True, 0.01, True, True)):
+        x, dout, dfinal = _inputs(3, *case)
+        got = _run(device, x, dout, dfinal, offset=1)
+        _check(got, *_wanted(x, dout, dfinal), case[4] + case[5] + case[0] / 8 + 256)
