@@ -308,3 +308,50 @@ def test_many_chunks_at_any_alignment(device):
         x, dout, dfinal = _inputs(3, *case)
         got = _run(device, x, dout, dfinal, offset=1)
         _check(got, *_wanted(x, dout, dfinal), case[4] + case[5] + case[0] / 8 + 256)
+
+
+def test_a_state_stepped_before_the_backward_is_refused(device):
+    """The backward reads the state that entered and, for the final state's
+    part of the decay's gradient, the one that left: a token step in place
+    between forward and backward must not spoil gradients in silence."""
+    from ttrl_amd.engine.autograd import Tensor, backward_from, no_grad
+    from ttrl_amd.engine.ops import linear_attention, linear_attention_step
+    from ttrl_amd.engine.tensor import DeviceArray
+
+    x, dout, dfinal = _inputs(50, 40, 2, 2, 2, 8, 8, True, None, True, True)
+    eager = _run(device, x, dout, dfinal)
+
+    def forward():
+        t = {n: _tensor(device, x[n], True) for n in ("q", "k", "v", "log_decay")}
+        both = DeviceArray(device, (2,) + x["state"].shape)  # two states of one allocation
+        both.upload(np.stack([x["state"]] * 2))
+        n = x["state"].size
+        t["state"], other = (Tensor(both.view(i * n, x["state"].shape)) for i in range(2))
+        out, final = linear_attention(*t.values())
+        return t, other, out, final, [(out, _tensor(device, dout, False)), (final, _tensor(device, dfinal, False))]
+
+    def act(state):
+        with no_grad():
+            linear_attention_step(*(_tensor(device, x[n][0], False) for n in ("q", "k", "v", "log_decay")), state)
+
+    t, other, out, final, seeds = forward()
+    act(t["state"])
+    with pytest.raises(RuntimeError, match="in place"):
+        backward_from(seeds)
+    t, other, out, final, seeds = forward()
+    act(Tensor(final.data))
+    with pytest.raises(RuntimeError, match="in place"):
+        backward_from(seeds)
+    # what the backward does not read may be stepped
+    t, other, out, final, seeds = forward()
+    act(other)
+    backward_from(seeds)
+    for n in ("q", "k", "v", "log_decay"):
+        assert np.array_equal(t[n].grad.numpy(), eager[n]), n
+    act(t["state"])  # and the state itself once it is done
+    t, other, out, final, seeds = forward()
+    act(Tensor(final.data))
+    backward_from(seeds[:1])
+    want, bound = _wanted(x, dout, None)
+    for n in ("q", "k", "v", "log_decay"):
+        _check({n: t[n].grad.numpy()}, {n: want[n]}, {n: bound[n]}, 8 + 8 + 5 + 256)

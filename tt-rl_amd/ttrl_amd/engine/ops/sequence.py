@@ -95,7 +95,11 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: 
     for a decay of each step; `state` (B, H, K, V) enters the first step
     (zeros when None); `done` (T, B, 1) resets the state entering a step
     where it is positive.  `scale` defaults to 1 / sqrt(K).
-    -> (outputs (T, B, H, V), final state (B, H, K, V)) as tape tensors."""
+    -> (outputs (T, B, H, V), final state (B, H, K, V)) as tape tensors.
+
+    The backward reads `state` and the final state where they are, as it reads
+    q, k and v: a state that goes on in `linear_attention_step` before the
+    backward has to be a copy, and the backward refuses one that was stepped."""
     (T, B), H, G, width, V, steps = _attention_shapes("linear_attention", q, k, v, log_decay, state, done, 2)
     dev = q.device
     d = _lib.LinearAttentionDesc()
@@ -118,9 +122,16 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: 
     outputs = Tensor(out, True, parents, "linear_attention")
     kept = (q.data, k.data, v.data, log_decay.data, state and state.data, done and done.data, saved, final)
     dfinal: list = []
+    before = (0 if state is None else state.data.steps_noted(), final.steps_noted())
 
     def _backward(grad: DeviceArray):
         _q, _k, _v, _g, _s, _d, _saved, _final = kept  # alive until here
+        if _s is not None and _s.steps_noted() != before[0]:
+            raise RuntimeError("linear_attention: the state that entered was stepped in place after the forward, and the "
+                               "backward reads it; step a copy")
+        if dfinal and log_decay.requires_grad and _final.steps_noted() != before[1]:
+            raise RuntimeError("linear_attention: the final state was stepped in place after the forward, and its part of "
+                               "the decay's gradient reads it; step a copy")
         grads = _Grads()
         work = DeviceArray(dev, (max(1, work_n),))
         arrays = [grads.array(t, t.shape, dev) for t in (q, k, v)]
@@ -151,7 +162,9 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     """One token of `linear_attention` for each of B lanes, as an acting step
     takes it: q (B, H, K), k (B, G, K), v (B, G, V), `log_decay` (1, H) or
     (B, H), `done` (B, 1).  `state` (B, H, K, V) is stepped in place;
-    -> the outputs (B, H, V).  Records no tape."""
+    -> the outputs (B, H, V).  Records no tape.  A backward that still has to
+    read `state` refuses to after this; replays of a captured step are not
+    seen, so there the caller keeps the two apart."""
     who = "linear_attention_step"
     (B,), H, G, width, V, rows = _attention_shapes(who, q, k, v, log_decay, state, done, 1)
     if state is None:
@@ -163,6 +176,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     dev.call("ttrl_linear_attention_token", B, H, G, width, V, q.data.vp, k.data.vp, v.data.vp, log_decay.data.vp,
              int(rows), _p(done), C.c_float(1.0 / math.sqrt(width) if scale is None else float(scale)), state.data.vp,
              out.vp)
+    state.data.note_step()
     return _detached(out)
 
 

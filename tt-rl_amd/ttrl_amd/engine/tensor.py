@@ -44,10 +44,11 @@ def _numel(shape) -> int:
 class _Block:
     """One allocation; frees itself when no DeviceArray refers to it."""
 
-    __slots__ = ("dev", "ptr", "nbytes", "__weakref__")
+    __slots__ = ("dev", "ptr", "nbytes", "steps", "__weakref__")
 
     def __init__(self, dev: Device, nbytes: int):
         self.dev = dev
+        self.steps = None
         self.nbytes = int(nbytes)
         self.ptr = dev.alloc(self.nbytes)
 
@@ -66,10 +67,11 @@ class _MappedBlock:
     host through `host.array` (a uint8 numpy view).  Frees itself with its
     last view."""
 
-    __slots__ = ("dev", "ptr", "nbytes", "host", "__weakref__")
+    __slots__ = ("dev", "ptr", "nbytes", "host", "steps", "__weakref__")
 
     def __init__(self, dev: Device, nbytes: int):
         self.dev = dev
+        self.steps = None
         self.host = dev.mapped_block(max(1, int(nbytes)))
         self.nbytes = self.host.nbytes
         self.ptr = self.host.dptr
@@ -132,6 +134,20 @@ class DeviceArray:
 
     def same_storage(self, other: "DeviceArray") -> bool:
         return self.block is other.block
+
+    # -- steps in place --------------------------------------------------------
+
+    def note_step(self) -> None:
+        """Counts a step of a recurrent state in place, over all of this array."""
+        if self.block.steps is None:
+            self.block.steps = {}
+        key = (self.offset, self.offset + self.nbytes)
+        self.block.steps[key] = self.block.steps.get(key, 0) + 1
+
+    def steps_noted(self) -> int:
+        """How many such steps have touched any of this array's memory."""
+        start, end = self.offset, self.offset + self.nbytes
+        return sum(n for (a, b), n in (self.block.steps or {}).items() if a < end and start < b)
 
     # -- transfer ------------------------------------------------------------
 
