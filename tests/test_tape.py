@@ -218,3 +218,17 @@ def test_capture_abort_lets_keyboard_interrupt_through(dev, monkeypatch):
     with pytest.raises(KeyboardInterrupt):
         capture(dev, record)
     assert rec.aborts == 1 and dev._capturing is False
+
+
+def test_a_seed_of_ones_that_is_added_to_is_no_seed_of_ones(dev):
+    """backward_from may give a node a gradient marked as all ones before a
+    kernel adds its own part in place: what the kernel writes to is not."""
+    from ttrl_amd.engine.tensor import DeviceArray
+
+    node = _node(dev, op="loss")
+    ones = DeviceArray(dev, (1, 1))
+    ones.fill(1.0)
+    assert ones.unit
+    node._accumulate(ones)
+    buf, beta = node._grad_target()
+    assert beta == 1.0 and buf is not ones and not buf.unit and ones.unit

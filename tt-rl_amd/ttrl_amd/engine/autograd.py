@@ -173,6 +173,7 @@ class Tensor:
             own.copy_from(self.grad)
             self.grad = own
             self._grad_owned = True
+        self.grad.unit = False  # ones that are added to
         return self.grad, 1.0
 
     def _note_write(self, beta: float, masked: bool):
