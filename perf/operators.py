@@ -141,6 +141,11 @@ def _gated_inputs(c, seed):
     t["b_gate"], t["b_up"] = ((_uniform(gen, bound, 1, c["hidden"]) if c["bias"] else None) for _ in range(2))
     if c["kind"] == "gated":
         t["dout"] = _normal(gen, c["rows"], c["hidden"])
+        if c["act"] == "relu":
+            # Relu's slope has no value where rounding decides the gate's sign: nothing is asked of such elements.
+            g = t["x"].double() @ t["w_gate"].double()
+            g = g if t["b_gate"] is None else g + t["b_gate"].double()
+            t["dout"].masked_fill_(g.abs() < 1e-4, 0.0)
     return t
 
 
