@@ -355,3 +355,21 @@ def test_a_state_stepped_before_the_backward_is_refused(device):
     want, bound = _wanted(x, dout, None)
     for n in ("q", "k", "v", "log_decay"):
         _check({n: t[n].grad.numpy()}, {n: want[n]}, {n: bound[n]}, 8 + 8 + 5 + 256)
+
+
+@pytest.mark.parametrize("T,B,resets,state", [(90, 57, None, False), (255, 8, 0.01, True), (1000, 256, 0.002, True), (1000, 2, None, True)])
+def test_a_shared_decay_of_short_memory(device, T, B, resets, state):
+    """The gradient of a decay that all steps share sums pairs of steps (i, j)
+    with a weight of i - j, a few steps where memory is short: rounding must not
+    be carried over the sequence instead.  Tolerance: every pair's terms are off
+    by K u and less in the mean (u = 2^-24), and what 32 steps sum of them may
+    cancel, so 32 + K of u times the root of the sum of squares of the steps'
+    terms |q . dq| + |k . dk|."""
+    K, V = 16, 16
+    x, dout, _ = _inputs(60, T, B, 1, 1, K, V, False, resets, state, False)
+    x["log_decay"][:] = np.log(0.75)
+    got = _run(device, x, dout, None)
+    want, _ = _wanted(x, dout, None)
+    term = np.abs(x["q"] * want["q"]).sum(-1) + np.abs(x["k"] * want["k"]).sum(-1)
+    err = abs(float(got["log_decay"][0, 0]) - float(want["log_decay"][0, 0]))
+    assert err <= (32 + K) * U * float(np.sqrt((term ** 2).sum())) + 2 * U * abs(float(want["log_decay"][0, 0]))
