@@ -845,8 +845,10 @@ int ttrl_gru_step_backward_ragged(ttrl_ctx* ctx, int B, int H, const float* dgh,
  * A step's q, k, v or outputs hold at most 2^24 values.
  * ttrl_linear_attention_space: floats of `saved`, which the forward fills for
  * the backward (forward_floats of it where no backward follows), and of
- * `work`, which the backward uses; each may be NULL where 0.  The backward overwrites dq, dk and dv (all required) and
- * dlog_decay unless NULL; with dlog_decay and dfinal it reads final_state. */
+ * `work`, which the backward uses; each may be NULL where 0.  The backward
+ * overwrites dq, dk and dv (all required) and dlog_decay unless NULL; it reads
+ * `state`, and with dlog_decay and dfinal final_state, as the forward had them:
+ * a token step between the two works on a copy. */
 typedef struct ttrl_linear_attention_desc {
   int T, B, H, kv_heads, K, V;
   const float* q;
@@ -884,7 +886,13 @@ int ttrl_linear_attention_token(ttrl_ctx* ctx, int B, int H, int kv_heads, int K
  * reference): h = act(x W_gate + b_gate) * (x W_up + b_up), x [M][K], weights
  * [K][N] (in, out), biases [N] or NULL, h [M][N].  g and u, both or neither,
  * receive the two projections for the backward.  Operands hold fewer than
- * 2^29 values.  act: */
+ * 2^29 values.
+ * Precision: forward products of up to 2^28 multiply-adds are FP32's.  Larger ones
+ * and the backward's are formed from two fp16 parts of each value, 22 bits, scaled
+ * by the largest value that shares its sums: a sum is off by at most 2^-21 + 2^-22
+ * of its terms' absolute values, beside FP32's own rounding, and where small
+ * values beside a large one could make it more it is formed in FP32.  NaN and
+ * infinity come out as FP32 has them.  act: */
 #define TTRL_GATE_SILU 0
 #define TTRL_GATE_GELU 1 /* with the error function */
 #define TTRL_GATE_RELU 2
@@ -925,7 +933,7 @@ int ttrl_gated_backward(ttrl_ctx* ctx, const ttrl_gated_desc* desc);
  * per element, and m_scale and v_scale [at / 64 ..] each block's largest
  * magnitude; m's code c stands for c |c| / 127^2 scale, v's for (c / 255)^4 scale;
  * the buffers hold whole blocks for every tensor.  A moment that is not
- * finite spoils its block.
+ * finite spoils its block: the scale holds it.
  * counter: TTRL_ADAMW_COUNTER_BYTES of device memory, set by
  * ttrl_adamw_set_count (t updates done) and moved on by every step. */
 #define TTRL_ADAMW_COUNTER_BYTES 2112

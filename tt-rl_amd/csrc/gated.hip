@@ -25,7 +25,7 @@
 // is off by 2^-21 at worst and 2^-24 in the mean, as one rounding of FP32 is;
 // every partial product is exact in FP32 and added in FP32, the sum rounded
 // three times per 32 k.  (Error against float64 at 8192 x 1024 x 4096: 1.1e-6 of
-// the largest, a library's FP32 products 1.7e-6.)  fp16 ends at 2^-24, so a
+// a gradient's norm, a library's FP32 products 1.7e-6.)  fp16 ends at 2^-24, so a
 // value under 2^-2 (2^-16 of its row's largest) is off by up to 2^-25 instead;
 // such values are counted by row, and every sum in which they could show (doubt()
 // and lossy_sums() below), or that is not finite, is formed again in FP32.  So a
@@ -34,7 +34,8 @@
 //
 // (Three bf16 parts, 24 bits at any exponent, need six products and no scale:
 // the forward and backward pass of 8192 x 1024 x 4096 took 2651 us so, 1546
-// with two fp16 parts in the same tiles, and 1368 to 1429 as it stands.)
+// with two fp16 parts in the same tiles, and 1424 to 1441 as it stands, 30 of
+// them for the guard against small values.)
 //
 // Operands are split once, by k_pack, into the very order in which the matrix
 // cores take them: 16 rows x 32 k of one part are 1 KiB,
@@ -43,8 +44,8 @@
 // reads them without conflicts, and every value is split once however many
 // tiles read it.  The scales cost one more pass over what is packed (k_scan);
 // packing writes 4 bytes a value beside the 4 read.  Where the time of that pass
-// goes (us): forward scan 13, pack 21, product 404; backward scan 120, pack 275
-// (1.1 GB, 4 TB/s), both products 604.
+// goes (us): forward scan 13, pack 25, product 439; backward scan 117, pack 268
+// (1.1 GB, 4 TB/s), both products 603.
 #include "tile_gemm.hpp"
 
 #include <algorithm>
@@ -133,8 +134,8 @@ __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(
 
 // The largest magnitudes of 32 x 128 values by row and by column.  NaN and
 // infinity count as the largest.  A wavefront has 8 rows, all (of slopes 4) in
-// flight.  Bound: memory (the backward's 470 MB 120 us, 3.9 TB/s), at 777 x 1333
-// the activations, 9 us (64 rows a tile: 21).
+// flight.  Bound: memory (the backward's 470 MB 117 us, 4.0 TB/s), at 777 x 1333
+// the activations, 10 us (64 rows a tile: 21).
 template <int ACT>  // of slopes; kNone: a plain matrix
 __device__ __forceinline__ void scan_tile(const PackJob& j, const Source& s, int tr, int tc, uint32_t (*top)[4][kScanC]) {
   constexpr bool SLOPES = ACT != kNone;
@@ -287,7 +288,7 @@ __device__ __forceinline__ void put_fragment(const Packed& to, int block, int st
 
 // A workgroup takes 32 x 64 values through LDS and writes them in both orders.
 // Bound: memory, 12 bytes read and 16 written for each pair of slopes (8192 x
-// 4096 with x and both weights: 275 us, 3.9 TB/s; a large copy 4.7).
+// 4096 with x and both weights: 268 us, 4.0 TB/s; a large copy 4.7).
 constexpr int kPackP = kPackC + 4;
 template <int ACT>
 __device__ __forceinline__ void pack_tile(const PackJob& j, const Source& s, int tr, int tc, float (*tile)[kPackR * kPackP]) {
@@ -619,11 +620,12 @@ __device__ __forceinline__ f32x4 plain_sums(const Source& s, long m, int n, int 
 }
 
 // WM x WN wavefronts of FM x FN fragments of 16 x 16, BUFS steps of operands in
-// LDS.  256 x 256 tiles run at 1.02 (forward, with the activation and three
+// LDS.  256 x 256 tiles run at 0.94 (forward, with the activation and three
 // outputs) and 1.37 PFLOP/s of fp16 (both gradients) at 8192 x 1024 x 4096; a
 // large bf16 product of the library 1.15.  Tiles of 256 x 128 were bound by the
-// L2s, which gave 9.7 TB/s (450 and 680 us, 404 and 604 with 256 x 256); reading
-// the next step's fragments while this one's products run took as long.
+// L2s, which gave 9.7 TB/s (450 and 680 us where 256 x 256 took 404 and 604, both
+// before sums were guarded one by one); reading the next step's fragments while
+// this one's products run took as long.
 // 64 x 64 tiles, three workgroups a compute unit, are as near the L2s' rate (9.4
 // TB/s at 777 x 500 x 1333); there a workgroup's 16 steps take 6 of 12 us, the
 // scales 2 and the results 2.5.
@@ -844,8 +846,10 @@ __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
 // 16 columns of both projections and 16 RB rows: the weights go from memory
 // into the products' registers, the wavefronts share K and their sums meet in
 // LDS, in order.  XV: x in whole 16-byte rows.  Bound: at one row the launch and
-// two memory round trips (512 x 2048, 8.4 MB of weights: 5.0 us, 1.7 TB/s), with
-// many the FP32 matrix rate.
+// two memory round trips (512 x 2048, 8.4 MB of weights: 5.0 us, 1.7 TB/s); with
+// more the weights' loads, 64 bytes of a row for each of 16 columns, dword by dword
+// (1024 x 4096 with 64 rows 18 us: 1.8 TB/s of weights, 59 TFLOP/s where a large
+// FP32 product runs at 153).
 struct FewArgs {
   const float *x, *wg, *wu;
   MmaArgs out;
@@ -931,8 +935,9 @@ long up_to(long n, long q) { return (n + q - 1) / q * q; }
 
 // Products that read their operands as they are: beyond, packing pays.  Forward
 // alone, calls one after another, this way and packed, us: K 512, N 2048 with 128
-// rows 9.9 / 25, 256 18 / 26, 512 32 / 29; 1024, 4096 with 32 13 / 36, 64 19 / 37, 192
-// 49 / 40; 2048, 1024 with 256 29 / 35, 300 53 / 38; 777 x 500 x 1333 51 / 37.
+// rows 9.4 / 27, 256 17 / 27, 512 32 / 30; 1024, 4096 with 32 13 / 38, 64 18 / 39, 192
+// 49 / 43; 2048, 1024 with 256 28 / 35, 300 53 / 38; 777 x 500 x 1333 43 / 34.  The line
+// is at 256 rows of the first, 64 of the second and 128 of the third.
 constexpr long kFewWork = 1L << 28;
 bool few_products(const ttrl_gated_desc* d) {
   return long(d->M) * d->K <= kFewWork / d->N && d->M <= 64 * 65535;  // 64 rows to each of a grid's y
@@ -941,9 +946,10 @@ bool few_products(const ttrl_gated_desc* d) {
 // A product's tiles and splits: 256 x 256 where they fill three quarters of the
 // compute units, counting what shares the launch, else 64 x 64, and k in splits
 // while there are fewer workgroups than two a compute unit and a split keeps
-// kMinSteps steps.  Both ways, us: 128 tiles of 256 x 256 at 2048 x 512 x 2048 205,
-// 64 x 64 158; at 8192 x 256 x 1024 259 and 227; at 8192 x 1024 x 4096 256 x 256 1429
-// and 256 x 128 1510.  128 x 64 took 94 at 777 x 500 x 1333, 64 x 64 92.
+// kMinSteps steps.  Forward alone in tiles of 256 x 256 and of 64 x 64, us: 128 tiles
+// (2048 x 512 x 2048) 81 / 57; 256 tiles 73 / 73 (8192 x 256 x 1024), 87 / 92 (4096 x 512
+// x 2048), 127 / 146 (4096 x 1024 x 2048); 512 tiles 159 / 163 (8192 x 512 x 2048); 1024
+// tiles 446 / 507 (8192 x 1024 x 4096).
 constexpr int kMinSteps = 6;
 struct MmaPlan {
   bool big;
