@@ -357,3 +357,18 @@ def test_packed_products_in_parts(device, M, K, N, act, bias):
 def test_packed_products_in_parts_at_any_alignment(device):
     x, dh = _inputs(42, 300, 1024, 1024, True)
     _check(_run(device, x, "silu", dh, 1), x, "silu", dh)
+
+
+def test_very_many_columns(device):
+    """More columns than a launch's threads count, forward; bias gradients of
+    more columns than are summed at once."""
+    from ttrl_amd.engine.autograd import no_grad
+    from ttrl_amd.engine.ops import gated_linear
+
+    N = (1 << 27) + 80
+    w = [np.resize(np.random.default_rng(s).standard_normal(100003).astype(np.float32), (1, N)) for s in (1, 2)]
+    with no_grad():
+        h = gated_linear(_tensor(device, np.float32([[0.5]])), *(_tensor(device, a) for a in w), activation="relu").numpy()
+    assert np.array_equal(h, np.maximum(np.float32(0.5) * w[0], 0) * (np.float32(0.5) * w[1]))
+    x, dh = _inputs(51, 40, 3, 40001, True)
+    _check(_run(device, x, "silu", dh), x, "silu", dh)

@@ -373,3 +373,35 @@ def test_a_shared_decay_of_short_memory(device, T, B, resets, state):
     term = np.abs(x["q"] * want["q"]).sum(-1) + np.abs(x["k"] * want["k"]).sum(-1)
     err = abs(float(got["log_decay"][0, 0]) - float(want["log_decay"][0, 0]))
     assert err <= (32 + K) * U * float(np.sqrt((term ** 2).sum())) + 2 * U * abs(float(want["log_decay"][0, 0]))
+
+
+def test_more_lanes_than_a_launch_counts(device):
+    """One step of more lanes and heads than a launch has workgroups of 256
+    threads for, with decays and resets, token by token and as a sequence."""
+    from ttrl_amd.engine.autograd import backward_from
+    from ttrl_amd.engine.ops import linear_attention, linear_attention_step
+
+    B = (1 << 24) + 70
+    rng = np.random.default_rng(70)
+
+    def normal(*s):
+        return np.resize(rng.standard_normal(100003).astype(np.float32), s)
+
+    q, k, v, s = normal(B, 1, 1), normal(B, 1, 1), normal(B, 1, 1), normal(B, 1, 1, 1)
+    g, done = np.full((1, 1), -0.5, np.float32), np.resize(np.float32([0, 0, 1]), (B, 1))
+    state = _tensor(device, s, False)
+    out = linear_attention_step(*(_tensor(device, a, False) for a in (q, k, v, g)), state, _tensor(device, done, False), scale=1.0)
+    keep = (np.float32(np.exp(np.float32(-0.5))) * (done <= 0))[..., None]
+    want = keep * s[..., 0] + k * v
+    size = np.abs(keep * s[..., 0]) + np.abs(k * v)
+    assert (np.abs(state.numpy()[..., 0] - want) <= 4 * U * size).all()
+    assert (np.abs(out.numpy() - q * want) <= 6 * U * np.abs(q) * size).all()
+
+    B = 1 << 24
+    x = {n: _tensor(device, a[:B].reshape((1,) * lead + a[:B].shape), True) for n, a, lead in
+         (("q", q, 1), ("k", k, 1), ("v", v, 1), ("state", s, 0))}
+    decay = _tensor(device, g, True)
+    out, _ = linear_attention(x["q"], x["k"], x["v"], decay, x["state"], _tensor(device, done[None, :B], False), scale=1.0)
+    backward_from([(out, _tensor(device, np.ones((1, B, 1, 1), np.float32), False))])
+    terms = (q * keep * s[..., 0])[:B].astype(np.float64)
+    assert abs(decay.grad.numpy()[0, 0] - terms.sum()) <= 64 * U * np.sqrt((terms ** 2).sum()) + 2 * U * abs(terms.sum())

@@ -788,7 +788,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mma(MmaPair pair) {
 // gradients, the column sums of every 32 rows in order.
 struct FinishArgs {
   MmaArgs job[2];
-  int blocks[2];  // workgroups of the products' splits; the rest sum columns
+  int blocks[2];  // workgroups of the products' splits
+  int columns;    // and of the column sums, 16 columns each in turn
   const float* sums;
   int tiles, N;
   float *db_gate, *db_up;
@@ -829,16 +830,21 @@ __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
     }
     block -= a.blocks[j];
   }
-  const int N = a.N, c = block * 16 + (threadIdx.x & 15), q = threadIdx.x >> 4;
-  double t = 0.0;
-  if (c < 2 * N)
-    for (int i = q; i < a.tiles; i += 16) t += double(a.sums[long(i) * 2 * N + c]);
-  red[threadIdx.x] = t;
-  __syncthreads();
-  if (q || c >= 2 * N) return;
-  for (int i = 1; i < 16; ++i) t += red[i * 16 + threadIdx.x];
-  float* to = c < N ? a.db_gate : a.db_up;
-  if (to) to[c < N ? c : c - N] = float(t);
+  const long N = a.N;
+  const int q = threadIdx.x >> 4;
+  for (long c = long(block) * 16 + (threadIdx.x & 15); c - (threadIdx.x & 15) < 2 * N; c += a.columns * 16L) {
+    double t = 0.0;
+    if (c < 2 * N)
+      for (int i = q; i < a.tiles; i += 16) t += double(a.sums[i * 2 * N + c]);
+    red[threadIdx.x] = t;
+    __syncthreads();
+    if (q == 0 && c < 2 * N) {
+      for (int i = 1; i < 16; ++i) t += red[i * 16 + threadIdx.x];
+      float* to = c < N ? a.db_gate : a.db_up;
+      if (to) to[c < N ? c : c - N] = float(t);
+    }
+    __syncthreads();
+  }
 }
 
 // ------------------------------------------------------- small products ---
@@ -853,15 +859,19 @@ __global__ __launch_bounds__(256) void k_finish(FinishArgs a) {
 struct FewArgs {
   const float *x, *wg, *wu;
   MmaArgs out;
+  int first;  // column that the launch begins with
 };
 constexpr int kFewWaves = 8;
+// Workgroups in x of one launch: its threads are counted in 32 bits, and a count
+// that passes them starts what is left of it without an error.
+constexpr int kFewGroups = 1 << 22;
 
 template <int RB, bool XV>
 __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
   __shared__ float part[kFewWaves][2 * RB * 256];
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int M = a.out.s.M, K = a.out.s.K, N = a.out.s.N, n = int(blockIdx.x) * 16 + lr;
+  const int M = a.out.s.M, K = a.out.s.K, N = a.out.s.N, n0 = a.first + int(blockIdx.x) * 16, n = n0 + lr;
   const __amdgpu_buffer_rsrc_t rx = make_res(a.x, uint32_t(M) * uint32_t(K) * 4u);
   const uint32_t bytes = uint32_t(K) * uint32_t(N) * 4u;
   const __amdgpu_buffer_rsrc_t rg = make_res(a.wg, bytes), ru = make_res(a.wu, bytes);
@@ -916,7 +926,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
       for (int r = 0; r < 4; ++r) part[wave][(q * RB + b) * 256 + (4 * lg + r) * 16 + lr] = acc[q][b][r];
   __syncthreads();
   for (int i = tid; i < RB * 256; i += 64 * kFewWaves) {
-    const int m = m0 + (i >> 4), c = int(blockIdx.x) * 16 + (i & 15);
+    const int m = m0 + (i >> 4), c = n0 + (i & 15);
     if (m >= M || c >= N) continue;
     float g = 0.f, u = 0.f;
 #pragma unroll
@@ -1100,7 +1110,7 @@ int launch_mma(ttrl_ctx* ctx, const MmaArgs* const* jobs, int count, bool big, c
 
 // Splits of the products that have any, and the bias gradients.
 int launch_finish(ttrl_ctx* ctx, const MmaArgs* const* jobs, int count, FinishArgs& a, const char* name) {
-  long blocks = a.sums ? ceil_div(2L * a.N, 16) : 0;
+  long blocks = a.columns = a.sums ? int(std::min(4096L, (2L * a.N + 15) / 16)) : 0;
   for (int i = 0; i < count; ++i) {
     const MmaArgs& m = *jobs[i];
     if (!m.part) continue;
@@ -1147,19 +1157,25 @@ int ttrl_gated_forward(ttrl_ctx* ctx, const ttrl_gated_desc* d) {
   m.o2 = d->u;
   m.s = source_of(d);
   if (few_products(d)) {
-    const FewArgs f{d->x, d->w_gate, d->w_up, m};
+    FewArgs f{d->x, d->w_gate, d->w_up, m, 0};
     const int rb = d->M <= 16 ? 1 : d->M <= 32 ? 2 : 4;
-    const dim3 grid(ceil_div(d->N, 16), ceil_div(d->M, 16 * rb)), block(64 * kFewWaves);
+    const int groups = ceil_div(d->N, 16);
+    const dim3 block(64 * kFewWaves);
     const bool xv = d->K % 4 == 0 && aligned16(d->x);
-    auto go = [&](auto rb) {
-      constexpr int RB = decltype(rb)::value;
-      if (xv) hipLaunchKernelGGL((k_few<RB, true>), grid, block, 0, stream_of(ctx), f);
-      else hipLaunchKernelGGL((k_few<RB, false>), grid, block, 0, stream_of(ctx), f);
-    };
-    if (rb == 1) go(std::integral_constant<int, 1>{});
-    else if (rb == 2) go(std::integral_constant<int, 2>{});
-    else go(std::integral_constant<int, 4>{});
-    return check_launch(name);
+    for (int from = 0; from < groups; from += kFewGroups) {
+      const dim3 grid(std::min(kFewGroups, groups - from), ceil_div(d->M, 16 * rb));
+      f.first = from * 16;
+      auto go = [&](auto rb) {
+        constexpr int RB = decltype(rb)::value;
+        if (xv) hipLaunchKernelGGL((k_few<RB, true>), grid, block, 0, stream_of(ctx), f);
+        else hipLaunchKernelGGL((k_few<RB, false>), grid, block, 0, stream_of(ctx), f);
+      };
+      if (rb == 1) go(std::integral_constant<int, 1>{});
+      else if (rb == 2) go(std::integral_constant<int, 2>{});
+      else go(std::integral_constant<int, 4>{});
+      if (int rc = check_launch(name)) return rc;
+    }
+    return TTRL_OK;
   }
   TTRL_REQUIRE(d->work && aligned16(d->work), "%s: null or unaligned workspace", name);
   const Layouts ls = layouts_of(d);

@@ -648,12 +648,12 @@ __global__ __launch_bounds__(kGradThreads) void k_decay_grad(SweepArgs a, const 
                                                              const float* __restrict__ final_grad, int DE,
                                                              const float* __restrict__ qd, const float* __restrict__ kd,
                                                              int parts, float* __restrict__ dg,
-                                                             double* __restrict__ sums) {
+                                                             double* __restrict__ sums, int first_bh) {
   constexpr int NWV = kGradThreads / 64, NC = kGradThreads / kChunk;
   __shared__ float red[NWV];
   __shared__ double first[NC], last[NC], part[NWV];
   __shared__ int whole[NC];
-  const long BH = long(a.B) * a.H, bh = blockIdx.x;
+  const long BH = long(a.B) * a.H, bh = first_bh + long(blockIdx.x);
   const int s = int(blockIdx.y), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = tid / kChunk, i = tid % kChunk;
   const int b = int(bh / a.H), h = int(bh - long(b) * a.H);
   const int t0 = s * a.seg, n = min(a.seg, a.T - t0), t = t0 + tid;
@@ -778,13 +778,14 @@ struct StepArgs {
   float *state, *out;
   int g_rows, B, H, share, K, V;
   float scale;
+  int first;  // head of a lane that the launch begins with
 };
 constexpr int kStepThreads = 256;
 
 template <int W>
 __global__ __launch_bounds__(kStepThreads) void k_token(StepArgs a) {
   __shared__ float part[kStepThreads * W];
-  const int bh = int(blockIdx.x), b = bh / a.H, h = bh - b * a.H, G = a.H / a.share;
+  const int bh = a.first + int(blockIdx.x), b = bh / a.H, h = bh - b * a.H, G = a.H / a.share;
   const int cols = (a.V + W - 1) / W, groups = kStepThreads / cols;
   const int c = int(threadIdx.x) % cols, kg = int(threadIdx.x) / cols;
   const float g = a.g_rows ? a.g[long(b) * a.H + h] : a.g[h];
@@ -834,6 +835,10 @@ __global__ __launch_bounds__(kStepThreads) void k_token(StepArgs a) {
 // ------------------------------------------------------------------ host ---
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Workgroups of 256 threads of one launch: its threads are counted in 32 bits, and
+// a count that passes them starts what is left of it without an error.
+constexpr long kMostGroups = 1L << 23;
 
 // Every row of the operand starts on 16 bytes.
 bool wide(const Operand& o) { return !o.p || (o.dim % 4 == 0 && aligned16(o.p)); }
@@ -1101,10 +1106,13 @@ int ttrl_linear_attention_backward(ttrl_ctx* ctx, const ttrl_linear_attention_de
   if (d->dlog_decay) {
     TTRL_REQUIRE(!d->dfinal || d->final_state, "%s: the final state's gradient needs the final state", name);
     double* total = d->decay_steps ? nullptr : reinterpret_cast<double*>(sums);
-    hipLaunchKernelGGL(k_decay_grad, dim3(unsigned(BH), unsigned(a.nseg)), dim3(kGradThreads), 0, stream_of(ctx), a,
-                       d->saved, grads, d->final_state, d->dfinal, int(DE), qdots, kdots, (d->K + 15) / 16,
-                       d->decay_steps ? d->dlog_decay : nullptr, total);
-    if (int rc = check_launch(name)) return rc;
+    for (long from = 0; from < BH; from += kMostGroups) {
+      const unsigned groups = unsigned(std::min(kMostGroups, BH - from));
+      hipLaunchKernelGGL(k_decay_grad, dim3(groups, unsigned(a.nseg)), dim3(kGradThreads), 0, stream_of(ctx), a, d->saved,
+                         grads, d->final_state, d->dfinal, int(DE), qdots, kdots, (d->K + 15) / 16,
+                         d->decay_steps ? d->dlog_decay : nullptr, total, int(from));
+      if (int rc = check_launch(name)) return rc;
+    }
     if (total) {
       hipLaunchKernelGGL(k_decay_total, dim3(unsigned(d->H)), dim3(64), 0, stream_of(ctx), total, d->H,
                          long(a.nseg) * d->B, d->dlog_decay);
@@ -1137,13 +1145,18 @@ int ttrl_linear_attention_token(ttrl_ctx* ctx, int B, int H, int kv_heads, int K
   TTRL_REQUIRE(long(B) * H <= 0x7fffffffL / 2, "%s: %d lanes of %d heads are too many", name, B, H);
   if (B == 0) return TTRL_OK;
   TTRL_REQUIRE(q && k && v && log_decay && state && out, "%s: null operand", name);
-  const StepArgs a{q, k, v, log_decay, done, state, out, decay_rows, B, H, H / kv_heads, K, V, scale};
-  const dim3 grid(unsigned(B) * unsigned(H));
-  if (V % 4 == 0 && aligned16(state) && aligned16(v))
-    hipLaunchKernelGGL(k_token<4>, grid, dim3(kStepThreads), 0, stream_of(ctx), a);
-  else
-    hipLaunchKernelGGL(k_token<1>, grid, dim3(kStepThreads), 0, stream_of(ctx), a);
-  return check_launch(name);
+  StepArgs a{q, k, v, log_decay, done, state, out, decay_rows, B, H, H / kv_heads, K, V, scale, 0};
+  const long BH = long(B) * H;
+  for (long from = 0; from < BH; from += kMostGroups) {
+    a.first = int(from);
+    const dim3 grid(unsigned(std::min(kMostGroups, BH - from)));
+    if (V % 4 == 0 && aligned16(state) && aligned16(v))
+      hipLaunchKernelGGL(k_token<4>, grid, dim3(kStepThreads), 0, stream_of(ctx), a);
+    else
+      hipLaunchKernelGGL(k_token<1>, grid, dim3(kStepThreads), 0, stream_of(ctx), a);
+    if (int rc = check_launch(name)) return rc;
+  }
+  return TTRL_OK;
 }
 
 }  // extern "C"
