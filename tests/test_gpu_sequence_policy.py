@@ -161,3 +161,19 @@ def test_the_recall_example_learns(device):
     assert result["losses"][-1] < 0.5 * result["losses"][0]
     assert result["recalled"] > 0.8  # a guess is right once in four
     assert result["difference"] <= 1e-4 * (1 + result["size"])
+
+
+def test_states_of_another_count_are_refused(device):
+    """A list with a state too few must not run fewer blocks in silence."""
+    from ttrl_amd.engine import Tensor, no_grad
+
+    policy, x, starts, states = _policy(device, SIZES[1])  # two blocks
+
+    def put(a):
+        return Tensor.from_numpy(a, device)
+
+    for wrong in ([put(states[0])], [put(s) for s in states + states[:1]], []):
+        with no_grad(), pytest.raises(ValueError, match="states"):
+            policy(put(x), wrong, put(starts))
+        with no_grad(), pytest.raises(ValueError, match="states"):
+            policy.step(put(x[0]), wrong, put(starts[0]))

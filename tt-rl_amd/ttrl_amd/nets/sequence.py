@@ -133,6 +133,12 @@ class SequencePolicy(Module):
     def initial_states(self, lanes: int) -> list:
         return [b.memory.initial_state(lanes) for b in self.blocks]
 
+    def _checked(self, states) -> list:
+        states = list(states)
+        if len(states) != len(self.blocks):
+            raise ValueError(f"SequencePolicy: {len(states)} states for {len(self.blocks)} blocks")
+        return states
+
     def _head(self, rows: Tensor) -> Tensor:
         return policy_value_packed(self.policy, self.critic, self.norm(rows))
 
@@ -143,7 +149,7 @@ class SequencePolicy(Module):
         rows = self.encoder(reshape(obs, (T * B, width)))
         x = reshape(rows, (T, B, _dims(rows)[1]))
         finals = []
-        for block, state in zip(self.blocks, states if states is not None else [None] * len(self.blocks)):
+        for block, state in zip(self.blocks, [None] * len(self.blocks) if states is None else self._checked(states)):
             x, final = block(x, state, starts)
             finals.append(final)
         return self._head(reshape(x, (T * B, _dims(rows)[1]))), finals
@@ -151,7 +157,7 @@ class SequencePolicy(Module):
     def step(self, obs: Tensor, states, starts: Tensor | None = None) -> Tensor:
         """One token for each lane, obs (B, obs_features): packed rows
         (B, n_actions + 1); `states` are stepped in place.  Inside no_grad()."""
-        x = self.encoder(obs)
+        states, x = self._checked(states), self.encoder(obs)
         for block, state in zip(self.blocks, states):
             x = block.step(x, state, starts)
         return self._head(x)
