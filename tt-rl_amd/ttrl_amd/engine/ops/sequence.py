@@ -183,7 +183,10 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
 def gated_linear(x: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Tensor | None = None, b_up: Tensor | None = None, *,
                  activation: str = "silu") -> Tensor:
     """act(x @ w_gate + b_gate) * (x @ w_up + b_up), both products, the
-    activation and their product in one launch; weights stored (in, out)."""
+    activation and their product in one kernel; weights stored (in, out).
+    Forward products of more than 2^28 multiply-adds and the gradients are
+    formed from operands of 22 bits (`ttrl_gated_desc` in ttrl_hip.h states
+    the bound), smaller ones in FP32."""
     who = "gated_linear"
     if activation not in _lib.GATES:
         raise ValueError(f"{who}: activation must be one of {list(GATED_ACTIVATIONS)}, got {activation!r}")
